@@ -309,6 +309,98 @@ W4A8_API w4a8_status w4a8_deltanet(const float* proj, const float* conv_w, float
                                    const uint32_t* params, int32_t nh, int32_t m, float eps, int32_t spec,
                                    void* stream);
 
+/* Paged KV cache of a batch of sequences, and the operators on it: the q/k norm with
+ * the rotation and the append (rope_kv.wgsl, qk_norm_rope.wgsl), attention of new tokens
+ * (attn.wgsl, attn_prefill.wgsl for one sequence and a contiguous cache), the weight that
+ * cached slots received, and eviction by that weight (the last two have no counterpart
+ * in the reference).
+ *
+ * Cache: k, v [pages, KVH, page, D] of type dtype, each with the strides page_stride,
+ * head_stride, row_stride (in elements, multiples of 8; unit inner stride; any order of
+ * the dimensions in memory, nothing overlapping), 16-byte aligned.  page: slots a page,
+ * a multiple of 16 up to 1024.  D: a multiple of 16 up to 256.  H query heads, H / KVH
+ * (at most 128) for each kv head, consecutive.
+ * Batch: sequence b has the new tokens q_start[b] .. q_start[b + 1] (q_start u32[batch + 1],
+ * q_start[0] = 0, at most `tokens` in all) and kv_len[b] slots, the new tokens' own among
+ * them: the last ones.  Slot j is row j % page of page table[b, j / page] (table
+ * u32[batch, table_stride]; entries past the length are not read).  New token i of n sees
+ * slots 0 .. kv_len - n + i, none where that is negative.  The arrays are read on the
+ * device, so a captured graph replays for new contents; the kernels bound every index
+ * taken from them (a start to tokens, a length to table_stride * page, a page to pages):
+ * a wrong entry gives wrong values and no access out of range.  max_q and max_kv bound
+ * the new tokens and slots of any sequence; what lies past them is not computed.  Slots
+ * past a sequence's length may hold anything, NaN too.  tokens = 0 is a no-op. */
+enum { W4A8_F16 = 0, W4A8_BF16 = 1, W4A8_F32 = 2 };
+
+/* Norm of queries and keys per head, rotation, and append to the cache, in one pass over
+ * the projection's rows: qkv f32, row t holds H query heads q_head_stride apart (D, or
+ * 2 D where each head's gate lies behind its query), then KVH key heads and KVH value
+ * heads of D.  Queries and keys: x / sqrt(mean(x^2) + eps) * w per head (q_norm, k_norm
+ * f32[D]; NULL skips the norm), then the first rot dims (a multiple of 16, 0 for none) turned by
+ * row pos[t] of rope f32[rope_rows, rot] (rot / 2 cosines, then rot / 2 sines; positions
+ * past the table take its last row): (a, b) -> (a cos - b sin, b cos + a sin) for the
+ * pairs (i, i + rot / 2), or (2i, 2i + 1) with interleaved.  q_out [tokens, H, D] of the
+ * cache's type; key and value of token i of n go to slot kv_len - n + i (nowhere where
+ * that is negative).  Values past f16's range become its largest value. */
+W4A8_API w4a8_status w4a8_qk_norm_rope_kv(const float* qkv, int32_t qkv_row_stride, int32_t q_head_stride, int32_t H,
+                                          int32_t KVH, int32_t D, const float* q_norm, const float* k_norm, float eps,
+                                          const float* rope, int32_t rot, int32_t rope_rows, int32_t interleaved,
+                                          const uint32_t* pos, const uint32_t* q_start, const uint32_t* kv_len,
+                                          const uint32_t* table, int32_t batch, int32_t table_stride, int32_t tokens,
+                                          void* q_out, void* k, void* v, int32_t dtype, int32_t pages, int32_t page,
+                                          size_t page_stride, int32_t head_stride, int32_t row_stride, void* stream);
+
+/* Attention of the batch's new tokens over the cache: softmax(scale q k^T) v over the
+ * slots each token sees, times sigmoid(gate) where gate is given.  q [tokens, H, D] of
+ * the cache's type, q_row_stride elements a token (a multiple of 8); gate f32, element
+ * t * gate_row_stride + h * gate_head_stride + d; o [tokens, H, D] of type o_type (the
+ * cache's, or W4A8_F32); lse f32[tokens, H] (natural log of the sum of exp(scale q k^T))
+ * or NULL.  A token that sees nothing gets o = 0 and lse = -inf.  Scores, sums and
+ * accumulators are f32; the weights are rounded to the cache's type before they
+ * meet v.  k and v must be finite in the slots below a sequence's length: a weight of
+ * zero times an infinity is NaN.
+ * workspace: w4a8_attn_paged_workspace_bytes(...) bytes, 16-byte aligned, any contents;
+ * calls that share one must not overlap on the GPU. */
+W4A8_API w4a8_status w4a8_attn_paged(const void* q, int32_t q_row_stride, int32_t H, int32_t KVH, int32_t D, float scale,
+                                     const float* gate, int32_t gate_row_stride, int32_t gate_head_stride,
+                                     const uint32_t* q_start, const uint32_t* kv_len, const uint32_t* table,
+                                     int32_t batch, int32_t table_stride, int32_t tokens, int32_t max_q, int32_t max_kv,
+                                     const void* k, const void* v, int32_t dtype, int32_t pages, int32_t page,
+                                     size_t page_stride, int32_t head_stride, int32_t row_stride, void* o, int32_t o_type,
+                                     float* lse, void* workspace, size_t workspace_bytes, void* stream);
+W4A8_API size_t w4a8_attn_paged_workspace_bytes(int32_t tokens, int32_t H, int32_t KVH, int32_t D, int32_t batch,
+                                                int32_t max_q, int32_t max_kv);
+
+/* The attention weight each slot received from the batch's new tokens, added to acc
+ * f32[batch, KVH, acc_stride] (acc_stride >= max_kv): acc[b, kvh, j] += the sum over
+ * the new tokens that see slot j and the query heads of kvh of exp(scale q k_j - lse), with
+ * q and lse as w4a8_attn_paged takes and gives them.  The same inputs give the same bits. */
+W4A8_API w4a8_status w4a8_attn_weights(const void* q, int32_t q_row_stride, const float* lse, int32_t H, int32_t KVH,
+                                       int32_t D, float scale, const uint32_t* q_start, const uint32_t* kv_len,
+                                       const uint32_t* table, int32_t batch, int32_t table_stride, int32_t tokens,
+                                       int32_t max_q, int32_t max_kv, const void* k, int32_t dtype, int32_t pages,
+                                       int32_t page, size_t page_stride, int32_t head_stride, int32_t row_stride,
+                                       float* acc, int32_t acc_stride, void* stream);
+
+/* Eviction by accumulated weight, for each sequence and kv head on its own: of len =
+ * kv_len[b] slots the n = min(len, keep[b]) stay that come first by (protected, weight
+ * acc, lower slot), NaN ranking as the lowest weight; a slot is protected where its
+ * token's position pos (u32[batch, KVH, stride], as acc) is below sink or at least
+ * protect_from[b].  The i-th kept slot at n or past it moves into the i-th dropped slot
+ * below n, K and V rows, weight and position; every other slot stays where it is
+ * (keys carry their rotation, so the order of slots has no meaning).  acc_out and pos_out
+ * get the first n entries of each head (they may be acc and pos); len_out[b] = n
+ * (not kv_len itself).  stride >= any kv_len.
+ * workspace: w4a8_kv_evict_workspace_bytes(...) bytes, 16-byte aligned, any contents;
+ * calls that share one must not overlap on the GPU. */
+W4A8_API w4a8_status w4a8_kv_evict(void* k, void* v, int32_t dtype, int32_t pages, int32_t page, size_t page_stride,
+                                   int32_t head_stride, int32_t row_stride, int32_t KVH, int32_t D,
+                                   const uint32_t* kv_len, const uint32_t* table, int32_t batch, int32_t table_stride,
+                                   const float* acc, const uint32_t* pos, int32_t stride, const uint32_t* keep,
+                                   const uint32_t* protect_from, int32_t sink, float* acc_out, uint32_t* pos_out,
+                                   uint32_t* len_out, void* workspace, size_t workspace_bytes, void* stream);
+W4A8_API size_t w4a8_kv_evict_workspace_bytes(int32_t batch, int32_t KVH, int32_t stride);
+
 /* Index carried by a packed argmax key (0 for the "no value > -3e38" key 0). */
 static inline uint32_t w4a8_key_index(uint64_t key) {
     return key ? ~(uint32_t)(key & 0xffffffffu) : 0u;

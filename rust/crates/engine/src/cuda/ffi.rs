@@ -48,6 +48,10 @@ pub const W4A8_STORE: i32 = 0;
 pub const W4A8_ADD: i32 = 1;
 pub const W4A8_SWIGLU: i32 = 2;
 
+pub const W4A8_F16: i32 = 0;
+pub const W4A8_BF16: i32 = 1;
+pub const W4A8_F32: i32 = 2;
+
 pub const W4A8_GEMV_MAX_M: i32 = 16;
 pub const W4A8_XCHG_HANDLE_BYTES: usize = 64;
 pub const W4A8_XCHG_MAX_RANKS: i32 = 8;
@@ -105,6 +109,35 @@ extern "C" {
     pub fn w4a8_deltanet(proj: *const f32, conv_w: *const f32, conv_state: *mut f32, state: *mut f32, out: *mut f32,
                          neg_a: *const f32, dt_bias: *const f32, gate_norm: *const f32, params: *const u32, nh: i32,
                          m: i32, eps: f32, spec: i32, stream: *mut c_void) -> w4a8_status;
+    pub fn w4a8_qk_norm_rope_kv(qkv: *const f32, qkv_row_stride: i32, q_head_stride: i32, h: i32, kvh: i32,
+                                d: i32, q_norm: *const f32, k_norm: *const f32, eps: f32, rope: *const f32,
+                                rot: i32, rope_rows: i32, interleaved: i32, pos: *const u32,
+                                q_start: *const u32, kv_len: *const u32, table: *const u32, batch: i32,
+                                table_stride: i32, tokens: i32, q_out: *mut c_void, k: *mut c_void,
+                                v: *mut c_void, dtype: i32, pages: i32, page: i32, page_stride: usize,
+                                head_stride: i32, row_stride: i32, stream: *mut c_void) -> w4a8_status;
+    pub fn w4a8_attn_paged(q: *const c_void, q_row_stride: i32, h: i32, kvh: i32, d: i32, scale: f32,
+                           gate: *const f32, gate_row_stride: i32, gate_head_stride: i32, q_start: *const u32,
+                           kv_len: *const u32, table: *const u32, batch: i32, table_stride: i32, tokens: i32,
+                           max_q: i32, max_kv: i32, k: *const c_void, v: *const c_void, dtype: i32, pages: i32,
+                           page: i32, page_stride: usize, head_stride: i32, row_stride: i32, o: *mut c_void,
+                           o_type: i32, lse: *mut f32, workspace: *mut c_void, workspace_bytes: usize,
+                           stream: *mut c_void) -> w4a8_status;
+    pub fn w4a8_attn_paged_workspace_bytes(tokens: i32, h: i32, kvh: i32, d: i32, batch: i32, max_q: i32,
+                                           max_kv: i32) -> usize;
+    pub fn w4a8_attn_weights(q: *const c_void, q_row_stride: i32, lse: *const f32, h: i32, kvh: i32, d: i32,
+                             scale: f32, q_start: *const u32, kv_len: *const u32, table: *const u32, batch: i32,
+                             table_stride: i32, tokens: i32, max_q: i32, max_kv: i32, k: *const c_void,
+                             dtype: i32, pages: i32, page: i32, page_stride: usize, head_stride: i32,
+                             row_stride: i32, acc: *mut f32, acc_stride: i32,
+                             stream: *mut c_void) -> w4a8_status;
+    pub fn w4a8_kv_evict(k: *mut c_void, v: *mut c_void, dtype: i32, pages: i32, page: i32, page_stride: usize,
+                         head_stride: i32, row_stride: i32, kvh: i32, d: i32, kv_len: *const u32,
+                         table: *const u32, batch: i32, table_stride: i32, acc: *const f32, pos: *const u32,
+                         stride: i32, keep: *const u32, protect_from: *const u32, sink: i32, acc_out: *mut f32,
+                         pos_out: *mut u32, len_out: *mut u32, workspace: *mut c_void, workspace_bytes: usize,
+                         stream: *mut c_void) -> w4a8_status;
+    pub fn w4a8_kv_evict_workspace_bytes(batch: i32, kvh: i32, stride: i32) -> usize;
     pub fn w4a8_group_dots(w: *const w4a8_weight, xq: *const i8, m: i32, dots: *mut i32,
                            stream: *mut c_void) -> w4a8_status;
     pub fn w4a8_gemm_group_dots(w: *const w4a8_weight, xq: *const i8, m: i32, dots: *mut i32,

@@ -13,6 +13,7 @@ OK, EINVAL, ECUDA, ENCCL, ETIMEOUT, ENOTSUP = range(6)
 STATUS_NAMES = {0: "OK", 1: "EINVAL", 2: "ECUDA", 3: "ENCCL", 4: "ETIMEOUT", 5: "ENOTSUP"}
 ACT_GROUP32, ACT_TOKEN = 0, 1
 STORE, ADD, SWIGLU = 0, 1, 2
+F16, BF16, F32 = 0, 1, 2
 GEMV_MAX_M = 16
 
 
@@ -57,6 +58,18 @@ _SIGS = {
     "w4a8_attn_decode": (ctypes.c_int, [_P, _P, _P, _I, _I, _I, _I, _P, _I, _I, _P, _P]),
     "w4a8_attn_combine": (ctypes.c_int, [_P, _I, _I, _I, _I, _P, _I, _P, _P, _P, _P, _P]),
     "w4a8_deltanet": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, ctypes.c_float, _I, _P]),
+    "w4a8_qk_norm_rope_kv": (ctypes.c_int, [_P, _I, _I, _I, _I, _I, _P, _P, ctypes.c_float, _P, _I, _I, _I, _P, _P,
+                                            _P, _P, _I, _I, _I, _P, _P, _P, _I, _I, _I, ctypes.c_size_t, _I, _I,
+                                            _P]),
+    "w4a8_attn_paged": (ctypes.c_int, [_P, _I, _I, _I, _I, ctypes.c_float, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I,
+                                       _I, _P, _P, _I, _I, _I, ctypes.c_size_t, _I, _I, _P, _I, _P, _P,
+                                       ctypes.c_size_t, _P]),
+    "w4a8_attn_paged_workspace_bytes": (ctypes.c_size_t, [_I, _I, _I, _I, _I, _I, _I]),
+    "w4a8_attn_weights": (ctypes.c_int, [_P, _I, _P, _I, _I, _I, ctypes.c_float, _P, _P, _P, _I, _I, _I, _I, _I, _P,
+                                         _I, _I, _I, ctypes.c_size_t, _I, _I, _P, _I, _P]),
+    "w4a8_kv_evict": (ctypes.c_int, [_P, _P, _I, _I, _I, ctypes.c_size_t, _I, _I, _I, _I, _P, _P, _I, _I, _P, _P,
+                                     _I, _P, _P, _I, _P, _P, _P, _P, ctypes.c_size_t, _P]),
+    "w4a8_kv_evict_workspace_bytes": (ctypes.c_size_t, [_I, _I, _I]),
     "w4a8_nccl_get_unique_id": (ctypes.c_int, [_P]),
     "w4a8_nccl_comm_init": (ctypes.c_int, [_I, _P, _I, ctypes.POINTER(ctypes.c_void_p)]),
     "w4a8_nccl_comm_destroy": (ctypes.c_int, [_P]),

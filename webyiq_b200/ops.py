@@ -8,6 +8,7 @@ checked by the library (W4A8Error with status EINVAL before any launch).
 """
 
 import ctypes
+import math
 
 import torch
 
@@ -288,6 +289,182 @@ def deltanet(proj, conv_w, conv_state, state, neg_a, dt_bias, gate_norm, params,
                                          _ptr(neg_a), _ptr(dt_bias), _ptr(gate_norm), _ptr(params), nh, m, eps,
                                          1 if spec else 0, _stream()))
     return out
+
+
+# ---------------------------------------------------------------------------
+# A batch of sequences over a paged KV cache (w4a8.h: the paged operators).
+
+_TYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+
+
+class PagedKV:
+    """A paged KV cache in device memory: k, v [pages, KVH, page, D], f16 or bf16, of the
+    same strides.  Any order of the dimensions in memory does (a cache stored [pages, page,
+    KVH, D] comes in as its permute(0, 2, 1, 3)); the inner stride is 1."""
+
+    def __init__(self, k, v):
+        if not (k.is_cuda and v.is_cuda) or k.device != v.device:
+            raise ValueError("PagedKV takes two tensors of one CUDA device")
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("PagedKV takes k and v [pages, KVH, page, D] of one type, float16 or bfloat16")
+        if k.stride() != v.stride() or k.stride(3) != 1:
+            raise ValueError("PagedKV takes k and v of the same strides, with inner stride 1")
+        self.k, self.v = k, v
+        self.pages, self.KVH, self.page, self.D = k.shape
+        self.dtype, self.device = k.dtype, k.device
+        self.layout = (_TYPES[k.dtype], self.pages, self.page, k.stride(0), k.stride(1), k.stride(2))
+        self.pk, self.pv = _ptr(k), _ptr(v)
+
+    def __repr__(self):
+        return f"PagedKV(pages={self.pages}, KVH={self.KVH}, page={self.page}, D={self.D}, {self.dtype})"
+
+
+class PagedBatch:
+    """A step's batch over a PagedKV: q_start int32 [B + 1] (first new token of each sequence,
+    from 0), kv_len int32 [B] (slots, the new tokens' own among them), table int32 [B, pages a
+    sequence].  max_q and max_kv bound the new tokens and the slots of any sequence (read on
+    the device otherwise, so the arrays may be rewritten in place between calls)."""
+
+    def __init__(self, q_start, kv_len, table, max_q, max_kv):
+        _need_cuda(q_start, kv_len, table)
+        self.B = kv_len.numel()
+        if q_start.dtype != torch.int32 or kv_len.dtype != torch.int32 or table.dtype != torch.int32:
+            raise ValueError("PagedBatch takes int32 tensors")
+        if q_start.numel() != self.B + 1 or table.dim() != 2 or table.shape[0] != self.B:
+            raise ValueError("PagedBatch takes q_start [B + 1], kv_len [B] and table [B, pages a sequence]")
+        self.q_start, self.kv_len, self.table = q_start, kv_len, table
+        self.max_q, self.max_kv = int(max_q), int(max_kv)
+        self.per = table.shape[1]
+        self.pq, self.pl, self.pt = _ptr(q_start), _ptr(kv_len), _ptr(table)
+
+
+def _need_rows(name, t, dtype, device):
+    """A [tokens, heads, D] tensor whose tokens may lie apart: (head, D) contiguous."""
+    if t.dtype != dtype or t.device != device or t.dim() != 3 or \
+            (t.numel() and (t.stride(2) != 1 or (t.stride(1) != t.shape[2] and t.shape[1] > 1))):
+        raise ValueError(f"{name}: a [tokens, heads, D] tensor of {dtype} on {device}, contiguous within a token")
+
+
+def qk_norm_rope_kv(qkv, kv, batch, pos, rope, H, q_norm=None, k_norm=None, eps=1e-6, gated=False, interleaved=False,
+                    q=None):
+    """Norms of q and k per head, rotation, and append of k and v to the cache (w4a8.h).
+    qkv f32 [tokens, (H + 2 KVH) D] (with gated, each query head followed by its gate: 2 H
+    heads of D in their place); pos int32 [tokens]; rope f32 [rows, rot] (cosines, then
+    sines) or None; q_norm, k_norm f32 [D] or None.  Returns q [tokens, H, D] of the
+    cache's type."""
+    _need_cuda(pos, rope, q_norm, k_norm, q)
+    if not qkv.is_cuda or qkv.dtype != torch.float32 or qkv.dim() != 2 or qkv.stride(1) != 1:
+        raise ValueError("qk_norm_rope_kv: qkv f32 [tokens, heads * D] with inner stride 1")
+    T, D = qkv.shape[0], kv.D
+    qhs = 2 * D if gated else D
+    if qkv.shape[1] != H * qhs + 2 * kv.KVH * D:
+        raise ValueError(f"qk_norm_rope_kv: rows of {qkv.shape[1]} for {H} query and {kv.KVH} kv heads of {D}")
+    for w in (q_norm, k_norm):
+        if w is not None and (w.dtype != torch.float32 or w.numel() != D):
+            raise ValueError("qk_norm_rope_kv: norm weights f32 [D]")
+    rot = rows = 0
+    if rope is not None:
+        if rope.dtype != torch.float32 or rope.dim() != 2 or pos is None or pos.dtype != torch.int32 or pos.numel() != T:
+            raise ValueError("qk_norm_rope_kv: rope f32 [rows, rot] and pos int32 [tokens]")
+        rows, rot = rope.shape
+    if q is None:
+        q = torch.empty((T, H, D), dtype=kv.dtype, device=qkv.device)
+    elif q.shape != (T, H, D) or q.dtype != kv.dtype:
+        raise ValueError("qk_norm_rope_kv: q [tokens, H, D] of the cache's type")
+    _lib.check(_lib.load().w4a8_qk_norm_rope_kv(
+        _ptr(qkv), qkv.stride(0) if T > 1 else qkv.shape[1], qhs, H, kv.KVH, D, _ptr(q_norm), _ptr(k_norm), eps,
+        _ptr(rope), rot, rows, interleaved, _ptr(pos), batch.pq, batch.pl, batch.pt, batch.B, batch.per, T, _ptr(q),
+        kv.pk, kv.pv, *kv.layout, _stream()))
+    return q
+
+
+def attn_paged_workspace(batch, tokens, H, KVH, D, device):
+    """Workspace of attn_paged for calls of up to this size (uint8; any contents)."""
+    n = _lib.load().w4a8_attn_paged_workspace_bytes(tokens, H, KVH, D, batch.B, batch.max_q, batch.max_kv)
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def attn_paged(q, kv, batch, scale=None, gate=None, o=None, lse=None, workspace=None):
+    """Attention of the new tokens over the cache (w4a8.h): q [tokens, H, D] of the cache's
+    type -> (o [tokens, H, D], lse f32 [tokens, H]); o of the cache's type, or f32 where
+    an f32 o is given; gate f32 [tokens, H, D] (any token and head stride): o times
+    sigmoid(gate).  scale defaults to 1 / sqrt(D)."""
+    _need_rows("attn_paged: q", q, kv.dtype, kv.device)
+    T, H, D = q.shape
+    if D != kv.D:
+        raise ValueError(f"attn_paged: q of {D} dims, a cache of {kv.D}")
+    _need_cuda(o, lse, workspace)
+    if o is None:
+        o = torch.empty((T, H, D), dtype=kv.dtype, device=q.device)
+    if lse is None:
+        lse = torch.empty((T, H), dtype=torch.float32, device=q.device)
+    if o.shape != q.shape or lse.numel() != T * H or lse.dtype != torch.float32:
+        raise ValueError("attn_paged: o [tokens, H, D], lse f32 [tokens, H]")
+    gr = gh = 0
+    if gate is not None:
+        if gate.dtype != torch.float32 or gate.shape != q.shape or gate.device != q.device or gate.stride(2) != 1:
+            raise ValueError("attn_paged: gate f32 [tokens, H, D] with inner stride 1")
+        gr, gh = gate.stride(0), gate.stride(1)
+    if workspace is None:
+        workspace = attn_paged_workspace(batch, T, H, kv.KVH, D, q.device)
+    _lib.check(_lib.load().w4a8_attn_paged(
+        _ptr(q), q.stride(0) if T > 1 else H * D, H, kv.KVH, D, 1.0 / math.sqrt(D) if scale is None else scale,
+        _ptr(gate), gr, gh, batch.pq, batch.pl, batch.pt, batch.B, batch.per, T, batch.max_q, batch.max_kv, kv.pk, kv.pv,
+        *kv.layout, _ptr(o), _TYPES.get(o.dtype, -1), _ptr(lse), _ptr(workspace), workspace.numel(), _stream()))
+    return o, lse
+
+
+def attn_weights(q, lse, kv, batch, acc, scale=None):
+    """acc f32 [B, KVH, slots] += the attention weight each slot received from the new
+    tokens (w4a8.h), with attn_paged's q, lse and scale.  Returns acc."""
+    _need_rows("attn_weights: q", q, kv.dtype, kv.device)
+    T, H, D = q.shape
+    _need_cuda(lse, acc)
+    if D != kv.D or lse.numel() != T * H or lse.dtype != torch.float32:
+        raise ValueError("attn_weights: q [tokens, H, D] of the cache's D, lse f32 [tokens, H]")
+    if acc.dtype != torch.float32 or acc.dim() != 3 or acc.shape[:2] != (batch.B, kv.KVH):
+        raise ValueError("attn_weights: acc f32 [B, KVH, slots]")
+    _lib.check(_lib.load().w4a8_attn_weights(
+        _ptr(q), q.stride(0) if T > 1 else H * D, _ptr(lse), H, kv.KVH, D,
+        1.0 / math.sqrt(D) if scale is None else scale, batch.pq, batch.pl, batch.pt, batch.B, batch.per, T,
+        batch.max_q, batch.max_kv, kv.pk, *kv.layout, _ptr(acc), acc.shape[2], _stream()))
+    return acc
+
+
+def kv_evict_workspace(batch, KVH, device, slots=None):
+    """Workspace of kv_evict (uint8; any contents) for acc and pos of `slots` entries a head;
+    where not given, enough for batch.max_kv slots rounded up to whole pages."""
+    n = _lib.load().w4a8_kv_evict_workspace_bytes(batch.B, KVH, batch.max_kv + 1024 if slots is None else slots)
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def kv_evict(kv, batch, acc, pos, keep, protect_from, sink=0, acc_out=None, pos_out=None, len_out=None, workspace=None):
+    """Eviction by accumulated weight (w4a8.h): of each sequence's slots keep[b] (int32) stay,
+    in place in the cache; acc f32 and pos int32 [B, KVH, slots].  Returns (acc_out, pos_out,
+    len_out): acc_out and pos_out default to acc and pos themselves, len_out to a new tensor
+    (it may not be batch.kv_len)."""
+    _need_cuda(acc, pos, keep, protect_from, acc_out, pos_out, len_out, workspace)
+    acc_out = acc if acc_out is None else acc_out
+    pos_out = pos if pos_out is None else pos_out
+    if len_out is None:
+        len_out = torch.empty_like(batch.kv_len)
+    if acc.dtype != torch.float32 or acc.dim() != 3 or acc.shape[:2] != (batch.B, kv.KVH) or pos.shape != acc.shape:
+        raise ValueError("kv_evict: acc f32 and pos int32 [B, KVH, slots]")
+    if acc_out.shape != acc.shape or pos_out.shape != acc.shape or acc_out.dtype != torch.float32:
+        raise ValueError("kv_evict: acc_out and pos_out as acc and pos")
+    for t, n in ((pos, 0), (pos_out, 0), (keep, batch.B), (protect_from, batch.B), (len_out, batch.B)):
+        if t.dtype != torch.int32 or (n and t.numel() != n):
+            raise ValueError("kv_evict: pos int32 as acc; keep, protect_from and len_out int32 [B]")
+    slots = acc.shape[2]
+    if slots < batch.max_kv:
+        raise ValueError(f"kv_evict: {slots} weights a head for up to {batch.max_kv} slots")
+    if workspace is None:
+        workspace = kv_evict_workspace(batch, kv.KVH, acc.device, slots)
+    _lib.check(_lib.load().w4a8_kv_evict(
+        kv.pk, kv.pv, *kv.layout, kv.KVH, kv.D, batch.pl, batch.pt, batch.B, batch.per, _ptr(acc), _ptr(pos), slots,
+        _ptr(keep), _ptr(protect_from), sink, _ptr(acc_out), _ptr(pos_out), _ptr(len_out), _ptr(workspace),
+        workspace.numel(), _stream()))
+    return acc_out, pos_out, len_out
 
 
 XCHG_HANDLE_BYTES = 64

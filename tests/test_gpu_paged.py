@@ -129,6 +129,49 @@ def test_attention_long(cuda, lens, news, H, KVH, D):
     c.check(*ops.attn_paged(c.q, c.kv, c.batch))
 
 
+def _dense(c, scale=None):
+    """Float64 attention on the GPU, one sequence and head at a time, for sizes past the restatement's."""
+    o = torch.zeros((c.T, c.H, c.D), dtype=torch.float64, device=c.cuda)
+    lse = torch.full((c.T, c.H), -torch.inf, dtype=torch.float64, device=c.cuda)
+    G = c.H // c.KVH
+    for b in range(c.B):
+        n, L = int(c.news[b]), int(c.lens[b])
+        if not n or not L:
+            continue
+        pg, row = (torch.from_numpy(x).to(c.cuda) for x in opg.slots(c.table, b, L, c.page))
+        k, v = c.k[pg, :, row].double(), c.v[pg, :, row].double()
+        t = slice(int(c.q_start[b]), int(c.q_start[b]) + n)
+        sees = torch.ones((n, L), dtype=torch.bool, device=c.cuda).tril(L - n)
+        for h in range(c.H):
+            s = (c.q[t, h].double() @ k[:, h // G].T / c.D ** 0.5).masked_fill(~sees, -torch.inf)
+            lse[t, h] = s.logsumexp(1)
+            o[t, h] = s.softmax(1).nan_to_num(0) @ v[:, h // G]
+    return o, lse
+
+
+@pytest.mark.parametrize("lens,news", [
+    ([100003], [1]), ([60001, 7, 30000], [1, 1, 2]), ([4001], [4001]), ([9000, 300], [1500, 300]),
+    ([100 + 37 * i for i in range(60)], [1] * 60), ([1 + i for i in range(300)], [1 + i % 3 for i in range(300)]),
+    ([2000 + 13 * i for i in range(12)], [(0, 1, 700, 90)[i % 4] for i in range(12)])])
+@pytest.mark.parametrize("H,KVH,D,dtype", [(8, 2, 256, "f16"), (32, 8, 128, "bf16"), (16, 1, 64, "f16"), (6, 2, 192, "bf16"),
+                                           (32, 2, 64, "bf16")])
+def test_attention_many_steps(cuda, lens, news, H, KVH, D, dtype):
+    """Stretches of many kv steps, items of one step, items that several CTAs share; against float64
+    on the same GPU, at the restatement's tolerances."""
+    c = Case(cuda, lens, news, H, KVH, D, dtype, page=32, seed=len(lens))
+    o, lse = ops.attn_paged(c.q, c.kv, c.batch)
+    assert ops.device_error() == 0
+    ro, rl = _dense(c)
+    vmax = c.v.float().nan_to_num(0).abs().max().item()
+    bad = (o.double() - ro).abs() > U[dtype] * (vmax + ro.abs()) + 2e-5 * vmax
+    assert not bad.any(), (int(bad.sum()), (o.double() - ro).abs().max().item())
+    assert torch.equal(torch.isneginf(lse), torch.isneginf(rl))
+    f = torch.isfinite(rl)
+    assert ((lse.double() - rl)[f].abs() <= 1e-5 * (1 + rl[f].abs())).all()
+    again = ops.attn_paged(c.q, c.kv, c.batch)
+    assert torch.equal(o, again[0]) and torch.equal(lse, again[1])
+
+
 def test_attention_gate_strides_types(cuda):
     """A gate beside each head's query, q inside a wider row, f32 output, another scale."""
     c = Case(cuda, [333, 20], [30, 1], 8, 2, 256, seed=9)

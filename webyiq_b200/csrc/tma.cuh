@@ -14,6 +14,7 @@ enum : unsigned int {
     DEV_ERR_GEMM_TIMEOUT = 2u,  // GEMM: a pipeline wait gave up
     DEV_ERR_SELFTEST = 4u,      // w4a8_selftest_wait_timeout: its wait gave up (as it must)
     DEV_ERR_XCHG_TIMEOUT = 8u,  // peer key exchange: a rank's flag never arrived
+    DEV_ERR_ATTN_TIMEOUT = 16u,  // paged attention or its weights: a pipeline wait gave up
 };
 
 // --- TMA bulk copies and mbarriers (no cluster multicast anywhere) -----------

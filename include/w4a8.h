@@ -359,11 +359,8 @@ W4A8_API w4a8_status w4a8_qk_norm_rope_kv(const float* qkv, int32_t qkv_row_stri
  * accumulators are f32; the weights are rounded to the cache's type before they
  * meet v.  k and v must be finite in the slots below a sequence's length: a weight of
  * zero times an infinity is NaN.
- * workspace: w4a8_attn_paged_workspace_bytes(...) bytes of the current device, 16-byte
- * aligned, zero-filled before its first use; every call leaves the counters in it zero
- * again (after a device error, fill it anew).  It may be larger than a call needs; the
- * arguments of one size may use it after another's.  Calls that share one must not
- * overlap on the GPU. */
+ * workspace: w4a8_attn_paged_workspace_bytes(...) bytes (of the current device), 16-byte
+ * aligned, any contents; calls that share one must not overlap on the GPU. */
 W4A8_API w4a8_status w4a8_attn_paged(const void* q, int32_t q_row_stride, int32_t H, int32_t KVH, int32_t D, float scale,
                                      const float* gate, int32_t gate_row_stride, int32_t gate_head_stride,
                                      const uint32_t* q_start, const uint32_t* kv_len, const uint32_t* table,

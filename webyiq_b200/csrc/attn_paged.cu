@@ -32,8 +32,9 @@
 // and each CTA takes an equal stretch of it, found on the device from the batch's
 // lengths: ragged batches, causal chunks and single long sequences all give every SM
 // the same number of steps.  An item that a stretch boundary cuts leaves partial (O,
-// max, sum) in the workspace; the CTA that finishes last merges them, in the order of
-// the stretches, so the result does not depend on which one that is.
+// max, sum) in the workspace, and a second, small kernel merges those, in the order of
+// the stretches (by the CTA that finishes last it took 28 us for one token over 10000
+// slots: one SM's threads, where the merge kernel has all of them).
 //
 // Warp roles: softmax warpgroups first (a warp reaches the tensor memory lanes of its
 // number modulo 4), then TMA, the two MMA warps (which also clear the V rows past a
@@ -53,6 +54,7 @@ constexpr uint32_t kChunkBytes = kTile * 128;  // 128 rows x 64 elements
 constexpr int kSegs = 4;
 constexpr int kMaxStages = 12;
 constexpr uint32_t kMiscBytes = 2048;
+constexpr int kItemCost = 2;  // an item's start and end (query load, epilogue), in kv steps
 constexpr float kLazy = 8.0f;  // log2 of how far the maximum may pass its reference
 
 struct AttnParams {
@@ -65,11 +67,12 @@ struct AttnParams {
     int o_type;
     float* lse;
     int max_q, max_kv;
-    int box_rows;  // slots of a TMA box
+    int box_rows;    // slots of a TMA box
+    int box_tokens;  // tokens of one
     CacheOrder order;
     int rows_cap;  // rows of a partial
-    uint32_t* counters;  // [CTA][NQ]
-    float* part;         // [CTA][2][NQ][rows_cap][D]
+    int4* shared_items;  // [CTA] the item that starts in its stretch and goes on in the next
+    float4* part;        // [CTA][2][NQ][D / 4][rows_cap]
     float2* ml;          // [CTA][2][NQ][rows_cap]
     unsigned int* err;
     PagedCache c;
@@ -105,9 +108,7 @@ struct Bars {
     uint64_t s_full[2], p_full[2], o_done[2];
     uint64_t q_full, q_empty;
     uint64_t seg_full[kSegs], seg_empty[kSegs];
-    uint64_t group[2];
     Segment seg[kSegs];
-    uint32_t last[2];
     uint32_t tmem;
     int abort;
 };
@@ -118,16 +119,159 @@ __device__ __forceinline__ int kv_steps(int vis_last, int len) {
     return max((end + kTile - 1) / kTile, 1);  // a tile that sees nothing still writes its zeros
 }
 
-// The batch as the work line sees it: new tokens and slots within the call's bounds.
-__device__ __forceinline__ SeqSpan line_span(const AttnParams& p, int seq) {
-    return seq_span(p.b, p.c, seq);
+// Length on the work line of one kv head of this lane's sequence (n tokens, 0 for none); a warp's call.
+// A sequence of many row tiles is summed by the whole warp.
+__device__ __forceinline__ int seq_length(const SeqSpan& s, int n, int tpc, int lane) {
+    int total = 0;
+    const bool many = n > 4 * tpc;
+    if (!many)
+        for (int i = 0; i < n; i += tpc) total += kv_steps(s.len - s.n + min(i + tpc, n) - 1, s.len) + kItemCost;
+    for (unsigned todo = __ballot_sync(kFull, many); todo; todo &= todo - 1) {
+        const int src = __ffs(todo) - 1;
+        const int n1 = __shfl_sync(kFull, n, src), len = __shfl_sync(kFull, s.len, src), sn = __shfl_sync(kFull, s.n, src);
+        int sum = 0;
+        for (int i = lane * tpc; i < n1; i += 32 * tpc) sum += kv_steps(len - sn + min(i + tpc, n1) - 1, len) + kItemCost;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
+        if (lane == src) total = sum;
+    }
+    return total;
 }
 
-// kv steps of one kv head of a sequence.
-__device__ __forceinline__ int seq_steps(const SeqSpan& s, int n, int tpc) {
-    int total = 0;
-    for (int i = 0; i < n; i += tpc) total += kv_steps(s.len - s.n + min(i + tpc, n) - 1, s.len);
-    return total;
+__device__ __forceinline__ void load_gate8(const AttnParams& p, int t, int h, int col, float4* g) {
+    const float4* at = reinterpret_cast<const float4*>(p.gate + static_cast<size_t>(t) * p.gate_row +
+                                                       static_cast<size_t>(h) * p.gate_head + col);
+    g[0] = ld_dep(at);
+    g[1] = ld_dep(at + 1);
+}
+// Eight columns of a row into the output: scaled, gated, rounded.
+template <typename T>
+__device__ __forceinline__ void put8(const AttnParams& p, int t, int h, int col, float* o, float f, const float4* gate) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= f;
+    if (p.gate) {
+        const float* g = reinterpret_cast<const float*>(gate);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = __fdividef(o[e], 1.f + __expf(-g[e]));
+    }
+    const size_t at = (static_cast<size_t>(t) * p.H + h) * p.D + col;
+    if (p.o_type == W4A8_F32) {
+        float4* d = reinterpret_cast<float4*>(static_cast<float*>(p.o) + at);
+        d[0] = make_float4(o[0], o[1], o[2], o[3]);
+        d[1] = make_float4(o[4], o[5], o[6], o[7]);
+    } else {
+        uint4 x;
+        x.x = Elem<T>::pack(Elem<T>::sat(o[0]), Elem<T>::sat(o[1]));
+        x.y = Elem<T>::pack(Elem<T>::sat(o[2]), Elem<T>::sat(o[3]));
+        x.z = Elem<T>::pack(Elem<T>::sat(o[4]), Elem<T>::sat(o[5]));
+        x.w = Elem<T>::pack(Elem<T>::sat(o[6]), Elem<T>::sat(o[7]));
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + at) = x;
+    }
+}
+
+// Where a CTA keeps its part of an item: the item that starts in its stretch in the
+// second place, the one that came over from the stretch before in the first.
+template <int NQ>
+__device__ __forceinline__ size_t part_slot(int cta, int first, int grp) {
+    return (static_cast<size_t>(cta) * 2 + (cta == first ? 1 : 0)) * NQ + grp;
+}
+
+// The merge of shared items.  Block (x, y): the item that starts in CTA x / NQ, row tile
+// x % NQ; the block's threads take 8 columns of a row each, split PG ways over the
+// item's parts.  Few rows (decode) have many parts and little else to go round, many
+// rows few parts.
+constexpr int kMergeThreads = 256;
+template <typename T, int NQ, int PG>
+__global__ void __launch_bounds__(kMergeThreads) attn_merge_kernel(const AttnParams p) {
+    constexpr int kE = kMergeThreads / PG;
+    __shared__ float red[PG > 1 ? kMergeThreads * 10 : 1];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int first = blockIdx.x / NQ, grp = blockIdx.x % NQ;
+    const int4 item = ld_dep(p.shared_items + first);
+    const int parts = item.w;
+    if (parts == 0) return;
+    const int rows = min(max(item.y - grp * p.tpt, 0), p.tpt) * p.G;
+    const int e = blockIdx.y * kE + threadIdx.x % kE, pg = threadIdx.x / kE;
+    const int col8 = e / p.rows_cap, row = e - col8 * p.rows_cap;
+    const bool live = col8 < p.D / 8 && row < rows;
+    const float c = p.scale * 1.44269504088896340736f;
+    float top = -INFINITY, sum = 0.f, o[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) o[x] = 0.f;
+    if (live) {
+        const size_t item_stride = static_cast<size_t>(p.D / 4) * p.rows_cap;
+        constexpr int kAhead = 4;
+        for (int q0 = pg; q0 < parts; q0 += PG * kAhead) {
+            float2 ml[kAhead];
+            float4 a[kAhead], b[kAhead];
+#pragma unroll
+            for (int x = 0; x < kAhead; ++x) {
+                const int q = q0 + x * PG;
+                ml[x] = make_float2(-INFINITY, 0.f);
+                a[x] = b[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (q < parts) {
+                    const size_t sl = part_slot<NQ>(first + q, first, grp);
+                    const float4* src = p.part + sl * item_stride + static_cast<size_t>(col8) * 2 * p.rows_cap + row;
+                    ml[x] = ld_dep(p.ml + sl * p.rows_cap + row);
+                    a[x] = ld_dep(src);
+                    b[x] = ld_dep(src + p.rows_cap);
+                }
+            }
+            float next = top;
+#pragma unroll
+            for (int x = 0; x < kAhead; ++x) next = fmaxf(next, ml[x].x);
+            const float keep = next == top ? 1.f : ex2((top - next) * c);
+            top = next;
+            sum *= keep;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) o[x] *= keep;
+#pragma unroll
+            for (int x = 0; x < kAhead; ++x) {
+                const float f = ml[x].x == top ? 1.f : ex2((ml[x].x - top) * c);
+                sum += f * ml[x].y;
+                o[0] += f * a[x].x;
+                o[1] += f * a[x].y;
+                o[2] += f * a[x].z;
+                o[3] += f * a[x].w;
+                o[4] += f * b[x].x;
+                o[5] += f * b[x].y;
+                o[6] += f * b[x].z;
+                o[7] += f * b[x].w;
+            }
+        }
+    }
+    if (PG > 1) {
+        // [value][thread]: the PG groups' partial results, merged by the first
+        red[threadIdx.x] = top;
+        red[kMergeThreads + threadIdx.x] = sum;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) red[(2 + x) * kMergeThreads + threadIdx.x] = o[x];
+        __syncthreads();
+        if (pg > 0) return;
+        float all = top;
+#pragma unroll
+        for (int q = 1; q < PG; ++q) all = fmaxf(all, red[q * kE + threadIdx.x]);
+        float f = top == all ? 1.f : ex2((top - all) * c);
+        sum *= f;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) o[x] *= f;
+#pragma unroll
+        for (int q = 1; q < PG; ++q) {
+            const int at = q * kE + threadIdx.x;
+            f = red[at] == all ? 1.f : ex2((red[at] - all) * c);
+            sum += f * red[kMergeThreads + at];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) o[x] += f * red[(2 + x) * kMergeThreads + at];
+        }
+        top = all;
+    }
+    if (!live) return;
+    const int t = item.x + grp * p.tpt + row / p.G, h = item.z * p.G + row % p.G;
+    float4 gate[2];
+    if (p.gate) load_gate8(p, t, h, col8 * 8, gate);
+    put8<T>(p, t, h, col8 * 8, o, sum == 0.f ? 0.f : 1.f / sum, gate);
+    if (col8 == 0 && p.lse) p.lse[static_cast<size_t>(t) * p.H + h] = sum == 0.f ? -INFINITY : top * p.scale + logf(sum);
 }
 
 template <typename T, int NCH, int NQ>
@@ -151,7 +295,6 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
             mbar_init(&bars.s_full[i], 1);
             mbar_init(&bars.p_full[i], 4);
             mbar_init(&bars.o_done[i], 1);
-            mbar_init(&bars.group[i], 128);
         }
         mbar_init(&bars.q_full, 1);
         mbar_init(&bars.q_empty, 2);
@@ -186,15 +329,19 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
         return s.j1 > 0;
     };
 
+    // NQ = 2: 384 threads of 168 registers; 256 x 200 + 128 x 104 is their sum
+    if (NQ == 2 && warp >= P::kSoftWarps) setmaxnreg_dec<104>();
     if (warp == kLineWarp) {
         // ---- the work line: this CTA's stretch of it, segment by segment ----
+        // kv steps of sequence b0 + lane, all its kv heads
+        auto steps_of = [&](int b0) {
+            SeqSpan s{};
+            if (b0 + lane < p.b.batch) s = seq_span(p.b, p.c, b0 + lane);
+            return static_cast<long long>(seq_length(s, min(s.n, p.max_q), tpc, lane)) * p.KVH;
+        };
         long long total = 0;
         for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
-            long long mine = 0;
-            if (b0 + lane < p.b.batch) {
-                const SeqSpan s = line_span(p, b0 + lane);
-                mine = static_cast<long long>(seq_steps(s, min(s.n, p.max_q), tpc)) * p.KVH;
-            }
+            long long mine = steps_of(b0);
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) mine += __shfl_xor_sync(kFull, mine, off);
             total += mine;
@@ -226,11 +373,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
         long long base = 0;
         if (at < end) {
             for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
-                long long mine = 0;
-                if (b0 + lane < p.b.batch) {
-                    const SeqSpan s = line_span(p, b0 + lane);
-                    mine = static_cast<long long>(seq_steps(s, min(s.n, p.max_q), tpc)) * p.KVH;
-                }
+                const long long mine = steps_of(b0);
                 long long upto = mine;
 #pragma unroll
                 for (int off = 1; off < 32; off <<= 1) {
@@ -251,18 +394,34 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
         int n = 0, kh = 0, i = 0, steps = 0;  // item: kv head kh, tokens from i
         long long item = base;                // its position
         if (at < end) {
-            s = line_span(p, seq);
+            s = seq_span(p.b, p.c, seq);
             n = min(s.n, p.max_q);
-            const long long per = seq_steps(s, n, tpc);
+            const long long per = __shfl_sync(kFull, seq_length(s, lane == 0 ? n : 0, tpc, lane), 0);
             kh = static_cast<int>((at - base) / per);
             item = base + kh * per;
-            for (;; i += tpc) {
-                steps = kv_steps(s.len - s.n + min(i + tpc, n) - 1, s.len);
-                if (item + steps > at) break;
-                item += steps;
+            for (;; i += 32 * tpc) {  // 32 row tiles at a time
+                const int first = i + lane * tpc;
+                steps = first < n ? kv_steps(s.len - s.n + min(first + tpc, n) - 1, s.len) : 0;
+                const int mine = first < n ? steps + kItemCost : 0;
+                int upto = mine;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) {
+                    const int y = __shfl_up_sync(kFull, upto, off);
+                    if (lane >= off) upto += y;
+                }
+                const unsigned past = __ballot_sync(kFull, item + upto > at);
+                if (past) {
+                    const int f = __ffs(past) - 1;
+                    i += f * tpc;
+                    item += __shfl_sync(kFull, upto - mine, f);
+                    steps = __shfl_sync(kFull, steps, f);
+                    break;
+                }
+                item += __shfl_sync(kFull, upto, 31);
             }
         }
-        while (at < end && ok) {
+        int4 shared_item = make_int4(0, 0, 0, 0);
+        while (item < end && ok) {
             Segment g;
             g.seq = seq;
             g.kh = kh;
@@ -270,13 +429,18 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
             g.n = min(tpc, n - i);
             g.vis = s.len - s.n + i;
             g.len = s.len;
-            g.j0 = static_cast<int>(at - item);
-            g.j1 = static_cast<int>(min(static_cast<long long>(steps), end - item));
-            g.first = cta_of(item);
-            g.parts = cta_of(item + steps - 1) - g.first + 1;
-            if (!publish(g)) break;
-            at += g.j1 - g.j0;
-            item += steps;
+            // the item's steps come behind its fixed cost
+            const long long start = item + kItemCost;
+            g.j0 = static_cast<int>(max(at - start, 0ll));
+            g.j1 = static_cast<int>(min(static_cast<long long>(steps), end - start));
+            g.first = cta_of(start);
+            g.parts = cta_of(start + steps - 1) - g.first + 1;
+            if (g.parts > 1 && g.first == static_cast<int>(blockIdx.x)) {
+                shared_item = make_int4(g.tok, g.n, g.kh, g.parts);
+            }
+            if (g.j1 > g.j0 && !publish(g)) break;
+            item += steps + kItemCost;
+            at = item;
             i += tpc;
             if (i >= n) {
                 i = 0;
@@ -284,13 +448,14 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                     kh = 0;
                     do {
                         if (++seq >= p.b.batch) break;
-                        s = line_span(p, seq);
+                        s = seq_span(p.b, p.c, seq);
                         n = min(s.n, p.max_q);
                     } while (n == 0);
                 }
             }
-            if (at < end) steps = kv_steps(s.len - s.n + min(i + tpc, n) - 1, s.len);
+            if (item < end) steps = kv_steps(s.len - s.n + min(i + tpc, n) - 1, s.len);
         }
+        if (lane == 0) p.shared_items[blockIdx.x] = shared_item;
         Segment stop{};
         if (ok) publish(stop);
     } else if (warp == kTmaWarp) {
@@ -346,7 +511,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                 break;
             }
             if (lane == 0) {
-                const uint32_t bytes = static_cast<uint32_t>(p.tpt) * p.G * 128;
+                const uint32_t bytes = static_cast<uint32_t>(p.box_tokens) * p.G * 128;
                 mbar_expect_tx(&bars.q_full, bytes * NCH * NQ);
                 for (int t = 0; t < NQ; ++t)
                     for (int ch = 0; ch < NCH; ++ch)
@@ -499,25 +664,21 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
         if (ok && have) pv(u - 1, first, valid);
     } else {
         // ---- softmax, one thread a row, and the output ----
+        if (NQ == 2) setmaxnreg_inc<200>();
+        constexpr int kOut = NQ == 2 ? 32 : 64;  // columns of O in registers at a time
         const int grp = NQ == 2 ? warp / 4 : 0;
         const int r = (warp & 3) * 32 + lane;  // row of the tile
         const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t o_tm = tmem + lane_off + kO + grp * NCH * 64;
         const float c = p.scale * 1.44269504088896340736f;
         const int tok_in = r / p.G, head_in = r - tok_in * p.G;
-        uint32_t u = 0, gphase = 0;  // units so far of this group
+        uint32_t u = 0;  // units so far of this group
         bool ok = true;
         // O after unit x of this group
         auto o_wait = [&](uint32_t x) {
             ok = !*bail.flag && bail.wait(&bars.o_done[NQ == 2 ? grp : (x & 1)], (NQ == 2 ? x : x >> 1) & 1);
             ok = __all_sync(kFull, ok);
             if (ok) tc1_fence_after();
-            return ok;
-        };
-        auto group_sync = [&]() {
-            mbar_arrive(&bars.group[grp]);
-            ok = bail.wait(&bars.group[grp], gphase & 1) && ok;
-            ++gphase;
             return ok;
         };
         Segment g;
@@ -529,6 +690,14 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
             int least = live ? lim : 0x7fffffff;
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) least = min(least, __shfl_xor_sync(kFull, least, off));
+            const int h = g.kh * p.G + head_in;
+            const int t = g.tok + grp * p.tpt + tok_in;
+            if (p.gate && live && g.parts == 1) {
+                // the gate is wanted at the segment's end: towards L2 now
+                const char* at = reinterpret_cast<const char*>(p.gate + static_cast<size_t>(t) * p.gate_row +
+                                                               static_cast<size_t>(h) * p.gate_head);
+                for (int e = 0; e < p.D * 4; e += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + e));
+            }
             float m = -INFINITY, l = 0.f;
             for (int j = g.j0; j < g.j1 && ok; ++j, ++u) {
                 const uint32_t buf = NQ == 2 ? grp : (u & 1), use = NQ == 2 ? u : u >> 1;
@@ -607,120 +776,48 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
             }
             if (!ok) break;
             if (!o_wait(u - 1)) break;
-            const int h = g.kh * p.G + head_in;
-            const int t = g.tok + grp * p.tpt + tok_in;
-            // 16 columns of a row into the output, scaled, gated, rounded
-            auto put = [&](int tt, int hh, int col, float* o, float f) {
-                if (p.gate) {
-                    const float4* gp = reinterpret_cast<const float4*>(p.gate + static_cast<size_t>(tt) * p.gate_row +
-                                                                       static_cast<size_t>(hh) * p.gate_head + col);
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        const float4 x = ld_dep(gp + e / 4);
-                        o[e] *= f / (1.f + __expf(-x.x));
-                        o[e + 1] *= f / (1.f + __expf(-x.y));
-                        o[e + 2] *= f / (1.f + __expf(-x.z));
-                        o[e + 3] *= f / (1.f + __expf(-x.w));
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] *= f;
-                }
-                const size_t at = (static_cast<size_t>(tt) * p.H + hh) * p.D + col;
-                if (p.o_type == W4A8_F32) {
-                    float4* d = reinterpret_cast<float4*>(static_cast<float*>(p.o) + at);
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4) d[e / 4] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                } else {
-                    uint4* d = reinterpret_cast<uint4*>(static_cast<T*>(p.o) + at);
-#pragma unroll
-                    for (int e = 0; e < 16; e += 8) {
-                        uint4 x;
-                        x.x = Elem<T>::pack(Elem<T>::sat(o[e]), Elem<T>::sat(o[e + 1]));
-                        x.y = Elem<T>::pack(Elem<T>::sat(o[e + 2]), Elem<T>::sat(o[e + 3]));
-                        x.z = Elem<T>::pack(Elem<T>::sat(o[e + 4]), Elem<T>::sat(o[e + 5]));
-                        x.w = Elem<T>::pack(Elem<T>::sat(o[e + 6]), Elem<T>::sat(o[e + 7]));
-                        d[e / 8] = x;
-                    }
-                }
-            };
             if (g.parts == 1) {
                 if (any_live) {
                     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
-                    for (int col = 0; col < p.D; col += 16) {
-                        float o[16];
-                        tmem1_ld16(o_tm + col, o);
+                    for (int col = 0; col < p.D; col += kOut) {
+                        // a chunk's gates are asked for at once: a load's latency a chunk, not a load
+                        float o[kOut];
+                        float4 gate[kOut / 4];
+                        if (p.gate && live)
+#pragma unroll
+                            for (int e = 0; e < kOut; e += 8)
+                                if (col + e < p.D) load_gate8(p, t, h, col + e, gate + e / 4);
+#pragma unroll
+                        for (int e = 0; e < kOut; e += 32) tmem1_ld32(o_tm + col + e, o + e);
                         tmem1_wait_ld();
-                        if (live) put(t, h, col, o, inv);
+                        if (live)
+#pragma unroll
+                            for (int e = 0; e < kOut; e += 8)
+                                if (col + e < p.D) put8<T>(p, t, h, col + e, o + e, inv, gate + e / 4);
                         __syncwarp();
                     }
                     if (live && p.lse) p.lse[static_cast<size_t>(t) * p.H + h] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
                 }
-                continue;
-            }
-            // a shared item: this CTA's part, then the merge by whoever comes last
-            const int rows = toks * p.G;
-            auto slot = [&](int cta) {
-                return (static_cast<size_t>(cta) * 2 + (cta == g.first ? 1 : 0)) * NQ + grp;
-            };
-            if (any_live) {
-                const size_t sl = slot(blockIdx.x);
-                float* dst = p.part + (sl * p.rows_cap + r) * p.D;
+            } else if (any_live) {
+                // a shared item: this CTA's part (neighbouring rows' 16 bytes lie side by side)
+                const size_t sl = part_slot<NQ>(blockIdx.x, g.first, grp);
+                float4* dst = p.part + sl * (p.D / 4) * p.rows_cap + r;
 #pragma unroll 1
-                for (int col = 0; col < p.D; col += 16) {
-                    float o[16];
-                    tmem1_ld16(o_tm + col, o);
+                for (int col = 0; col < p.D; col += 32) {
+                    float o[32];
+                    tmem1_ld32(o_tm + col, o);
                     tmem1_wait_ld();
                     if (live) {
 #pragma unroll
-                        for (int e = 0; e < 16; e += 4)
-                            __stcg(reinterpret_cast<float4*>(dst + col + e), make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+                        for (int e = 0; e < 32; e += 4)
+                            if (col + e < p.D) dst[static_cast<size_t>((col + e) / 4) * p.rows_cap] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                     }
                     __syncwarp();
                 }
-                if (live) __stcg(p.ml + sl * p.rows_cap + r, make_float2(m, l));
+                if (live) p.ml[sl * p.rows_cap + r] = make_float2(m, l);
             }
             tc1_fence_before();
-            __threadfence();
-            if (!group_sync()) break;
-            const int gt = threadIdx.x & 127;
-            uint32_t* counter = p.counters + static_cast<size_t>(g.first) * NQ + grp;
-            if (gt == 0) {
-                const uint32_t before = atomicAdd(counter, 1u);
-                bars.last[grp] = before == static_cast<uint32_t>(g.parts - 1);
-                if (before == static_cast<uint32_t>(g.parts - 1)) *counter = 0;
-                __threadfence();
-            }
-            if (!group_sync()) break;
-            if (!bars.last[grp]) continue;
-            for (int e = gt; e < rows * (p.D / 16); e += 128) {
-                const int row = e / (p.D / 16), col = (e - row * (p.D / 16)) * 16;
-                float top = -INFINITY;
-                for (int q = 0; q < g.parts; ++q) top = fmaxf(top, __ldcg(p.ml + slot(g.first + q) * p.rows_cap + row).x);
-                float o[16], sum = 0.f;
-#pragma unroll
-                for (int x = 0; x < 16; ++x) o[x] = 0.f;
-                for (int q = 0; q < g.parts; ++q) {
-                    const size_t sl = slot(g.first + q);
-                    const float2 ml = __ldcg(p.ml + sl * p.rows_cap + row);
-                    const float f = ml.x == top ? 1.f : ex2((ml.x - top) * c);
-                    sum += f * ml.y;
-                    const float4* src = reinterpret_cast<const float4*>(p.part + (sl * p.rows_cap + row) * p.D + col);
-#pragma unroll
-                    for (int x = 0; x < 16; x += 4) {
-                        const float4 v = __ldcg(src + x / 4);
-                        o[x] += f * v.x;
-                        o[x + 1] += f * v.y;
-                        o[x + 2] += f * v.z;
-                        o[x + 3] += f * v.w;
-                    }
-                }
-                const int tt = g.tok + grp * p.tpt + row / p.G, hh = g.kh * p.G + row % p.G;
-                put(tt, hh, col, o, sum == 0.f ? 0.f : 1.f / sum);
-                if (col == 0 && p.lse)
-                    p.lse[static_cast<size_t>(tt) * p.H + hh] = sum == 0.f ? -INFINITY : top * p.scale + logf(sum);
-            }
         }
     }
 
@@ -804,7 +901,7 @@ namespace {
 // How a call is laid out on the GPU, from its sizes alone.
 struct Layout {
     int nch, nq, tpt, rows_cap, grid;
-    size_t counters, slots, bytes;
+    size_t items, slots, bytes;
 };
 
 Layout layout_of(int H, int KVH, int D, int batch, int max_q, int max_kv, int sms) {
@@ -817,12 +914,11 @@ Layout layout_of(int H, int KVH, int D, int batch, int max_q, int max_kv, int sm
     x.rows_cap = std::min(x.tpt, std::max(max_q, 1)) * G;
     const long long tiles = (static_cast<long long>(std::max(max_q, 1)) + x.nq * x.tpt - 1) / (x.nq * x.tpt);
     const long long steps = std::max((static_cast<long long>(max_kv) + kTile - 1) / kTile, 1ll);
-    const long long work = std::min(tiles * steps, 1ll << 20) * KVH * batch;
+    const long long work = std::min(tiles * (steps + kItemCost), 1ll << 20) * KVH * batch;  // the longest the line can be
     x.grid = static_cast<int>(std::min<long long>(sms, work));
-    // the same place and size whatever the call, so that calls of several sizes may share a workspace
-    x.counters = (static_cast<size_t>(sms) * 2 * 4 + 255) / 256 * 256;
+    x.items = (static_cast<size_t>(x.grid) * 16 + 255) / 256 * 256;
     x.slots = static_cast<size_t>(x.grid) * 2 * x.nq * x.rows_cap;
-    x.bytes = x.counters + (x.slots * 8 + 255) / 256 * 256 + x.slots * D * 4;
+    x.bytes = x.items + (x.slots * 8 + 255) / 256 * 256 + x.slots * D * 4;
     return x;
 }
 
@@ -834,7 +930,18 @@ w4a8_status launch_tc(const CUtensorMap& q, const CUtensorMap& k, const CUtensor
     static FuncAttr attr;
     const w4a8_status s = ensure_smem(attn_tc_kernel<T, NCH, NQ>, attr, Pl::kSmem, -1, what);
     if (s != W4A8_OK) return s;
-    return launch_pdl(what, attn_tc_kernel<T, NCH, NQ>, dim3(grid), dim3(Pl::kThreads), Pl::kSmem, st, q, k, v, p);
+    const w4a8_status r =
+        launch_pdl(what, attn_tc_kernel<T, NCH, NQ>, dim3(grid), dim3(Pl::kThreads), Pl::kSmem, st, q, k, v, p);
+    if (r != W4A8_OK || grid == 1) return r;
+    // by how many threads a row's 8 columns are shared: about as many as fill the GPU for two items
+    const int work = p.rows_cap * (p.D / 8);
+    auto merge = [&](auto kernel, int pg) {
+        const int per = kMergeThreads / pg;
+        return launch_pdl(what, kernel, dim3(grid * NQ, (work + per - 1) / per), dim3(kMergeThreads), 0, st, p);
+    };
+    if (work <= 512) return merge(attn_merge_kernel<T, NQ, 16>, 16);
+    if (work <= 2048) return merge(attn_merge_kernel<T, NQ, 4>, 4);
+    return merge(attn_merge_kernel<T, NQ, 1>, 1);
 }
 
 template <typename T>
@@ -915,13 +1022,14 @@ W4A8_API w4a8_status w4a8_attn_paged(const void* q, int32_t q_row_stride, int32_
     p.max_q = max_q;
     p.max_kv = max_kv;
     p.box_rows = cache_box_rows(page);
+    p.box_tokens = std::min(x.tpt, max_q);
     p.rows_cap = x.rows_cap;
-    p.counters = static_cast<uint32_t*>(workspace);
-    p.ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + x.counters);
-    p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + x.counters + (x.slots * 8 + 255) / 256 * 256);
+    p.shared_items = static_cast<int4*>(workspace);
+    p.ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + x.items);
+    p.part = reinterpret_cast<float4*>(static_cast<char*>(workspace) + x.items + (x.slots * 8 + 255) / 256 * 256);
     p.err = device_error_word();
     CUtensorMap mq, mk, mv;
-    st = encode_queries(&mq, q, dtype, H, D, q_row_stride, tokens, p.G, x.tpt, what);
+    st = encode_queries(&mq, q, dtype, H, D, q_row_stride, tokens, p.G, p.box_tokens, what);
     if (st == W4A8_OK) st = encode_cache(&mk, &p.order, k, p.c, KVH, D, what);
     if (st == W4A8_OK) st = encode_cache(&mv, &p.order, v, p.c, KVH, D, what);
     if (st != W4A8_OK) return st;

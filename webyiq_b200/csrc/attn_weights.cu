@@ -4,80 +4,445 @@
 //   acc[b, kvh, j] += sum over new tokens i that see j, query heads h of kvh, of
 //                     exp(scale q_ih . k_j - lse_ih)
 //
-// The sum over rows belongs to one CTA for each slot, in a fixed order: no atomics, and
-// the same inputs give the same bits.
+// The scores come from the tensor cores the other way round, S^T = K Q^T: a tile's 128
+// slots are the MMA's M (a tensor memory lane and a thread each), the query rows (token
+// * G + head) its N.  So a slot's sum over rows stays in one thread, in a fixed order:
+// no atomics and no shuffles, the same bits every time.  The exponent's offset is per
+// column, read from shared memory (one broadcast load for four).
+//
+// An item is one tile of slots of a kv head; it stays in shared memory while the query
+// rows that see it pass.  Items lie on a line weighted by their row tiles (plus one for
+// the tile itself), and each CTA takes those that start in an equal stretch of it, found
+// on the device from the batch's lengths.  Single tokens are bound by HBM (K is read
+// once), chunks by the exponentials: 128 x 128 of them take the SM's 16 a clock 1024
+// clocks, the MMA half of that at 128-wide heads.
+//
+// Warp roles: two softmax warpgroups that take row tiles in turn (four S buffers, so
+// the MMAs run ahead), then TMA, MMA, and the warp that walks the line.
 #include "launch.cuh"
-#include "paged.cuh"
+#include "tc_f16.cuh"
 
 namespace w4a8 {
 
 namespace {
 
-constexpr int kRows = 16, kKeys = 32, kThreads = 128;
+constexpr int kTile = 128;
+constexpr uint32_t kChunkBytes = kTile * 128;  // 128 rows x 64 elements
+constexpr int kKRing = 7, kQRing = 6;          // 16 KB chunks of slots and of query rows
+constexpr int kSBufs = 4, kItems = 4;
+constexpr int kSoftWarps = 8, kThreads = (kSoftWarps + 4) * 32;
 
 struct WeightParams {
-    const void* q;
-    int q_row, H, KVH, D;
+    int H, KVH, G, nch;
+    int tpt;         // tokens of a row tile
+    int box_tokens;  // tokens that one load of query rows brings
+    int cols;        // N of the MMA: box_tokens * G rounded up to 16
     float scale;
     const float* lse;
     float* acc;
     int acc_stride, max_q;
+    int box_rows;
+    CacheOrder order;
+    unsigned int* err;
     PagedCache c;
     PagedBatch b;
 };
 
+struct Item {
+    int seq, kh;
+    int t0, n;      // the sequence's first new token (global) and how many
+    int vis;        // last slot its first new token sees
+    int len, j;     // slots, and the tile's number
+    int i0, steps;  // first row tile that sees the tile's first slot, and how many from it; steps == 0: the end
+};
+
+struct Smem {
+    unsigned char k[kKRing][kChunkBytes];
+    unsigned char q[kQRing][kChunkBytes];
+    float off[2][2][kTile];  // [group][turn][column]: -lse * log2 e
+    float sum[2][kTile];     // the second group's sums of an item, on the way to the first
+    uint64_t k_full[kKRing], k_empty[kKRing], q_full[kQRing], q_empty[kQRing];
+    uint64_t s_full[kSBufs], s_empty[kSBufs];
+    uint64_t item_full[kItems], item_empty[kItems];
+    uint64_t group[2], sum_full[2], sum_empty[2];
+    Item item[kItems];
+    uint32_t tmem;
+    int abort;
+};
+constexpr size_t kSmemBytes = 1024 + sizeof(Smem);
+static_assert(kSmemBytes <= 227 * 1024, "shared memory plan exceeds 227 KB");
+
+// First row tile of a sequence that sees slot tile j (the rows before it see none of it).
+__device__ __forceinline__ int first_row_tile(const SeqSpan& s, int j, int tpt) {
+    return max(0, j * kTile - (s.len - s.n)) / tpt;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) weights_rows_kernel(const WeightParams p) {
-    extern __shared__ float sm[];
+__global__ void __launch_bounds__(kThreads, 1)
+    weights_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                      const WeightParams p) {
+    extern __shared__ unsigned char smem_raw[];
+    Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kTmaWarp = kSoftWarps, kMmaWarp = kTmaWarp + 1, kLineWarp = kTmaWarp + 2;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kKRing; ++i) {
+            mbar_init(&sm.k_full[i], 1);
+            mbar_init(&sm.k_empty[i], 1);
+        }
+        for (int i = 0; i < kQRing; ++i) {
+            mbar_init(&sm.q_full[i], 1);
+            mbar_init(&sm.q_empty[i], 1);
+        }
+        for (int i = 0; i < kSBufs; ++i) {
+            mbar_init(&sm.s_full[i], 1);
+            mbar_init(&sm.s_empty[i], 4);
+        }
+        for (int i = 0; i < kItems; ++i) {
+            mbar_init(&sm.item_full[i], 1);
+            mbar_init(&sm.item_empty[i], kSoftWarps + 2);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm.group[i], 128);
+            mbar_init(&sm.sum_full[i], 4);
+            mbar_init(&sm.sum_empty[i], 4);
+        }
+        sm.abort = 0;
+        mbar_init_fence();
+    }
+    if (warp == kMmaWarp) tmem1_alloc(&sm.tmem, 512);
+    tc1_fence_before();
+    __syncthreads();
+    tc1_fence_after();
+    const uint32_t tmem = sm.tmem;
     pdl_launch_dependents();
     pdl_wait();
-    const int G = p.H / p.KVH, D = p.D, ld = D + 1;
-    const int seq = blockIdx.z, kh = blockIdx.y, j0 = blockIdx.x * kKeys;
-    const SeqSpan sp = seq_span(p.b, p.c, seq);
-    const int rows = min(sp.n, p.max_q) * G;
-    const int len = min(sp.len, p.acc_stride);
-    if (j0 >= len || rows == 0) return;
-    float* qs = sm;               // [16][D + 1]
-    float* ks = qs + kRows * ld;  // [32][D + 1]
-    float* ps = ks + kKeys * ld;  // [16][33]
-    const int tid = threadIdx.x;
-    for (int e = tid; e < kKeys * D; e += kThreads) {
-        const int j = j0 + e / D, d = e % D;
-        ks[(e / D) * ld + d] =
-            j < len ? static_cast<float>(ld_dep(static_cast<const T*>(p.c.k) + slot_offset(p.b, p.c, seq, kh, j) + d)) : 0.f;
-    }
-    float total = 0.f;
-    for (int r0 = 0; r0 < rows; r0 += kRows) {
-        __syncthreads();
-        for (int e = tid; e < kRows * D; e += kThreads) {
-            const int r = e / D, d = e % D, rr = min(r0 + r, rows - 1);
-            const size_t at = static_cast<size_t>(sp.t0 + rr / G) * p.q_row + static_cast<size_t>(kh * G + rr % G) * D + d;
-            qs[r * ld + d] = static_cast<float>(ld_dep(static_cast<const T*>(p.q) + at)) * p.scale;
-        }
-        __syncthreads();
-        for (int e = tid; e < kRows * kKeys; e += kThreads) {
-            const int r = e / kKeys, j = e % kKeys;
-            float w = 0.f;
-            if (r0 + r < rows && j0 + j < len && j0 + j <= sp.len - sp.n + (r0 + r) / G) {
-                float s = 0.f;
-                for (int d = 0; d < D; ++d) s += qs[r * ld + d] * ks[j * ld + d];
-                const int t = sp.t0 + (r0 + r) / G, h = kh * G + (r0 + r) % G;
-                w = expf(s - ld_dep(p.lse + static_cast<size_t>(t) * p.H + h));
+
+    const Bail bail{&sm.abort, p.err};
+    uint32_t items = 0;
+    auto next_item = [&](Item& it) -> bool {
+        const uint32_t i = items % kItems;
+        const bool ok = !*bail.flag && bail.wait(&sm.item_full[i], (items / kItems) & 1);
+        if (!__all_sync(kFull, ok)) return false;
+        it = sm.item[i];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.item_empty[i]);
+        ++items;
+        return it.steps > 0;
+    };
+
+    if (warp == kLineWarp) {
+        // ---- the line of items: an item's length is its row tiles and one for its slots ----
+        // new tokens and slot tiles of sequence b; none where either is none
+        auto span = [&](int b, SeqSpan& s, int& n, int& tiles) {
+            s = b < p.b.batch ? seq_span(p.b, p.c, b) : SeqSpan{};
+            n = min(s.n, p.max_q);
+            tiles = n > 0 ? (min(s.len, p.acc_stride) + kTile - 1) / kTile : 0;
+        };
+        auto item_len = [&](const SeqSpan& s, int n, int j) {
+            return max((n + p.tpt - 1) / p.tpt - first_row_tile(s, j, p.tpt), 0) + 1;
+        };
+        // length of one kv head of this lane's sequence
+        auto seq_len = [&](const SeqSpan& s, int n, int tiles) {
+            const bool many = n > p.tpt || n < s.n;
+            int total = tiles * 2;  // one row tile, which sees something of every slot tile
+            for (unsigned todo = __ballot_sync(kFull, many); todo; todo &= todo - 1) {
+                const int src = __ffs(todo) - 1;
+                SeqSpan o;
+                o.t0 = 0;
+                o.n = __shfl_sync(kFull, s.n, src);
+                o.len = __shfl_sync(kFull, s.len, src);
+                const int on = __shfl_sync(kFull, n, src), ot = __shfl_sync(kFull, tiles, src);
+                int sum = 0;
+                for (int j = lane; j < ot; j += 32) sum += item_len(o, on, j);
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
+                if (lane == src) total = sum;
             }
-            ps[r * 33 + j] = w;
+            return total;
+        };
+        SeqSpan s;
+        int n, tiles;
+        long long total = 0;
+        for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
+            span(b0 + lane, s, n, tiles);
+            long long mine = static_cast<long long>(seq_len(s, n, tiles)) * p.KVH;
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) mine += __shfl_xor_sync(kFull, mine, off);
+            total += mine;
         }
-        __syncthreads();
-        if (tid < kKeys) {
-            float s = 0.f;
-            for (int r = 0; r < kRows; ++r) s += ps[r * 33 + tid];
-            total += s;
+        const long long at = blockIdx.x * total / gridDim.x, end = (blockIdx.x + 1) * total / gridDim.x;
+        int seq = 0, kh = 0, j = 0;
+        long long pos = 0;  // start of item (seq, kh, j)
+        bool ok = true;
+        if (at < end) {
+            for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
+                span(b0 + lane, s, n, tiles);
+                const long long mine = static_cast<long long>(seq_len(s, n, tiles)) * p.KVH;
+                long long upto = mine;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) {
+                    const long long y = __shfl_up_sync(kFull, upto, off);
+                    if (lane >= off) upto += y;
+                }
+                const unsigned past = __ballot_sync(kFull, pos + upto > at);
+                if (past) {
+                    const int f = __ffs(past) - 1;
+                    seq = b0 + f;
+                    pos += __shfl_sync(kFull, upto - mine, f);
+                    const long long per = __shfl_sync(kFull, mine, f) / p.KVH;
+                    kh = static_cast<int>((at - pos) / per);
+                    pos += kh * per;
+                    break;
+                }
+                pos += __shfl_sync(kFull, upto, 31);
+            }
+            span(seq, s, n, tiles);
+            // the first item that starts at `at` or past it
+            for (int j0 = 0; j0 < tiles; j0 += 32) {
+                const int len = j0 + lane < tiles ? item_len(s, n, j0 + lane) : 0;
+                int upto = len;
+#pragma unroll
+                for (int off = 1; off < 32; off <<= 1) {
+                    const int y = __shfl_up_sync(kFull, upto, off);
+                    if (lane >= off) upto += y;
+                }
+                const unsigned past = __ballot_sync(kFull, j0 + lane < tiles && pos + upto - len >= at);
+                if (past) {
+                    const int f = __ffs(past) - 1;
+                    j = j0 + f;
+                    pos += __shfl_sync(kFull, upto - len, f);
+                    break;
+                }
+                j = min(j0 + 32, tiles);
+                pos += __shfl_sync(kFull, upto, 31);
+            }
+        }
+        uint32_t sent = 0;
+        auto publish = [&](const Item& it) {
+            const uint32_t i = sent % kItems;
+            ok = ok && !*bail.flag && bail.wait(&sm.item_empty[i], ((sent / kItems) & 1) ^ 1);
+            if (!__all_sync(kFull, ok)) return ok = false;
+            if (lane == 0) {
+                sm.item[i] = it;
+                mbar_arrive(&sm.item_full[i]);
+            }
+            ++sent;
+            return true;
+        };
+        while (ok && at < end) {
+            if (j >= tiles) {  // the next kv head or sequence
+                j = 0;
+                if (++kh == p.KVH) {
+                    kh = 0;
+                    do {
+                        if (++seq >= p.b.batch) break;
+                        span(seq, s, n, tiles);
+                    } while (tiles == 0);
+                    if (seq >= p.b.batch) break;
+                }
+            }
+            if (pos >= end) break;
+            Item it;
+            it.seq = seq;
+            it.kh = kh;
+            it.t0 = s.t0;
+            it.n = n;
+            it.vis = s.len - s.n;
+            it.len = min(s.len, p.acc_stride);
+            it.j = j;
+            it.i0 = first_row_tile(s, j, p.tpt);
+            it.steps = (n + p.tpt - 1) / p.tpt - it.i0;
+            if (it.steps > 0) publish(it);
+            pos += max(it.steps, 0) + 1;
+            ++j;
+        }
+        Item stop{};
+        if (ok) publish(stop);
+    } else if (warp == kTmaWarp) {
+        // ---- TMA: the item's slots, then the query rows, chunk by chunk ----
+        const int boxes = kTile / p.box_rows;
+        const uint32_t box_bytes = static_cast<uint32_t>(p.box_rows) * 128;
+        const uint32_t q_bytes = static_cast<uint32_t>(p.box_tokens) * p.G * 128;
+        uint32_t kn = 0, qn = 0;
+        bool ok = true;
+        Item it;
+        while (ok && next_item(it)) {
+            const int s0 = it.j * kTile + lane * p.box_rows;
+            const int n = min(boxes, (it.len - it.j * kTile + p.box_rows - 1) / p.box_rows);
+            int page = 0, row = 0;
+            if (lane < n) {
+                const int pi = s0 / p.c.page;
+                page = static_cast<int>(page_of(p.b, p.c, it.seq, pi));
+                row = s0 - pi * p.c.page;
+            }
+            for (int ch = 0; ch < p.nch && ok; ++ch, ++kn) {
+                const uint32_t st = kn % kKRing;
+                ok = !*bail.flag && bail.wait(&sm.k_empty[st], ((kn / kKRing) & 1) ^ 1);
+                if (!(ok = __all_sync(kFull, ok))) break;
+                if (lane == 0) mbar_expect_tx(&sm.k_full[st], static_cast<uint32_t>(n) * box_bytes);
+                __syncwarp();
+                if (lane < n)
+                    tma_load_4d(smem_u32(sm.k[st]) + lane * box_bytes, &tm_k, ch * 64, p.order.pick(0, row, it.kh, page),
+                                p.order.pick(1, row, it.kh, page), p.order.pick(2, row, it.kh, page), &sm.k_full[st]);
+            }
+            for (int i = it.i0; i < it.i0 + it.steps && ok; ++i) {
+                for (int ch = 0; ch < p.nch && ok; ++ch, ++qn) {
+                    const uint32_t st = qn % kQRing;
+                    ok = !*bail.flag && bail.wait(&sm.q_empty[st], ((qn / kQRing) & 1) ^ 1);
+                    if (!(ok = __all_sync(kFull, ok))) break;
+                    if (lane == 0) {
+                        mbar_expect_tx(&sm.q_full[st], q_bytes);
+                        tma_load_3d_at(smem_u32(sm.q[st]), &tm_q, ch * 64, it.kh * p.G, it.t0 + i * p.tpt, &sm.q_full[st]);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        // no copy may still be landing when the CTA exits
+        for (uint32_t x = kn > kKRing ? kn - kKRing : 0; x < kn; ++x) mbar_wait(&sm.k_full[x % kKRing], (x / kKRing) & 1);
+        for (uint32_t x = qn > kQRing ? qn - kQRing : 0; x < qn; ++x) mbar_wait(&sm.q_full[x % kQRing], (x / kQRing) & 1);
+    } else if (warp == kMmaWarp) {
+        // ---- MMA: S^T = K Q^T per row tile ----
+        const uint32_t idesc = idesc_f16<T>(0, false) | (static_cast<uint32_t>(p.cols >> 3) << 17);
+        uint32_t kn = 0, qn = 0, sn = 0;
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            ok = ok && !*bail.flag && bail.wait(bar, parity);
+            return ok = __all_sync(kFull, ok);
+        };
+        Item it;
+        while (ok && next_item(it)) {
+            for (int i = 0; i < it.steps && ok; ++i, ++sn) {
+                const uint32_t buf = sn % kSBufs;
+                if (!wait(&sm.s_empty[buf], ((sn / kSBufs) & 1) ^ 1)) break;
+                for (int ch = 0; ch < p.nch; ++ch) {
+                    const uint32_t ks = (kn + ch) % kKRing, qs = (qn + ch) % kQRing;
+                    if (i == 0 && !wait(&sm.k_full[ks], ((kn + ch) / kKRing) & 1)) break;
+                    if (!wait(&sm.q_full[qs], ((qn + ch) / kQRing) & 1)) break;
+                    tc1_fence_after();
+                    if (lane == 0) {
+                        const uint32_t ka = smem_u32(sm.k[ks]), qa = smem_u32(sm.q[qs]);
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            mma_f16_ss(tmem + buf * kTile, desc_k_major(ka + kk * 32), desc_k_major(qa + kk * 32), idesc,
+                                       ch + kk > 0);
+                        tc1_commit(&sm.q_empty[qs]);
+                        if (i == it.steps - 1) tc1_commit(&sm.k_empty[ks]);
+                    }
+                    __syncwarp();
+                }
+                if (lane == 0) tc1_commit(&sm.s_full[buf]);
+                __syncwarp();
+                qn += p.nch;
+            }
+            kn += p.nch;
+        }
+    } else if (warp < kSoftWarps) {
+        // ---- exponentials and sums, one thread a slot ----
+        const int grp = warp >> 2, gt = threadIdx.x & 127;
+        const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const float c = p.scale * 1.44269504088896340736f;
+        const float2 c2 = make_float2(c, c);
+        const int tok_in = gt / p.G, head_in = gt - tok_in * p.G;  // this thread's column when offsets are fetched
+        uint32_t sn = 0, turn = 0, done = 0;
+        bool ok = true;
+        Item it;
+        while (ok && next_item(it)) {
+            const int slot = it.j * kTile + gt;
+            float total = 0.f;
+            for (int i = 0; i < it.steps && ok; ++i, ++sn) {
+                if (static_cast<int>(sn & 1) != grp) continue;
+                const int tok0 = (it.i0 + i) * p.tpt;
+                const int toks = min(it.n - tok0, p.tpt);
+                // offsets of the tile's columns, for the whole group
+                float* off = sm.off[grp][turn & 1];
+                float mine = 0.f;
+                if (tok_in < toks)
+                    mine = ld_dep(p.lse + static_cast<size_t>(it.t0 + tok0 + tok_in) * p.H + it.kh * p.G + head_in) *
+                           -1.44269504088896340736f;
+                off[gt] = mine;
+                mbar_arrive(&sm.group[grp]);
+                ok = !*bail.flag && bail.wait(&sm.group[grp], turn & 1);
+                ++turn;
+                const uint32_t buf = sn % kSBufs;
+                ok = ok && !*bail.flag && bail.wait(&sm.s_full[buf], (sn / kSBufs) & 1);
+                if (!(ok = __all_sync(kFull, ok))) break;
+                tc1_fence_after();
+                const uint32_t s_tm = tmem + lane_off + buf * kTile;
+                const int cols = toks * p.G;
+                // the first column that sees this slot
+                const int lo = max(slot - (it.vis + tok0), 0) * p.G;
+                // every slot of the warp is seen by every column, and every column is live
+                const bool all = __all_sync(kFull, lo == 0) && cols % 32 == 0;
+                float2 a0 = make_float2(0.f, 0.f), a1 = make_float2(0.f, 0.f);
+                for (int x = 0; x < cols; x += 32) {
+                    float s[32];
+                    if (x + 32 <= p.cols) {
+                        tmem1_ld32(s_tm + x, s);
+                    } else {  // 16 columns: the MMA wrote no more
+                        tmem1_ld16(s_tm + x, s);
+#pragma unroll
+                        for (int e = 16; e < 32; ++e) s[e] = 0.f;
+                    }
+                    tmem1_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 o = *reinterpret_cast<const float4*>(off + x + e);
+                        float2 u = __ffma2_rn(make_float2(s[e], s[e + 1]), c2, make_float2(o.x, o.y));
+                        float2 v = __ffma2_rn(make_float2(s[e + 2], s[e + 3]), c2, make_float2(o.z, o.w));
+                        u.x = ex2(u.x);
+                        u.y = ex2(u.y);
+                        v.x = ex2(v.x);
+                        v.y = ex2(v.y);
+                        if (!all) {
+                            const int q = x + e;
+                            u.x = q >= lo && q < cols ? u.x : 0.f;
+                            u.y = q + 1 >= lo && q + 1 < cols ? u.y : 0.f;
+                            v.x = q + 2 >= lo && q + 2 < cols ? v.x : 0.f;
+                            v.y = q + 3 >= lo && q + 3 < cols ? v.y : 0.f;
+                        }
+                        a0 = __fadd2_rn(a0, u);
+                        a1 = __fadd2_rn(a1, v);
+                    }
+                }
+                total += (a0.x + a0.y) + (a1.x + a1.y);
+                tc1_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.s_empty[buf]);
+            }
+            if (!ok) break;
+            // the second group hands its share of the item to the first
+            const uint32_t d = done & 1, phase = (done >> 1) & 1;
+            ++done;
+            ok = !*bail.flag && bail.wait(grp == 1 ? &sm.sum_empty[d] : &sm.sum_full[d], grp == 1 ? phase ^ 1 : phase);
+            if (!(ok = __all_sync(kFull, ok))) break;
+            if (grp == 1)
+                sm.sum[d][gt] = total;
+            else
+                total += sm.sum[d][gt];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(grp == 1 ? &sm.sum_full[d] : &sm.sum_empty[d]);
+            if (grp == 0 && slot < it.len) {
+                float* at = p.acc + (static_cast<size_t>(it.seq) * p.KVH + it.kh) * p.acc_stride + slot;
+                *at = ld_dep(at) + total;
+            }
         }
     }
-    if (tid < kKeys && j0 + tid < len)
-        p.acc[(static_cast<size_t>(seq) * p.KVH + kh) * p.acc_stride + j0 + tid] += total;
+
+    tc1_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc1_fence_after();
+        tmem1_dealloc(tmem, 512);
+    }
 }
 
 }  // namespace
+
+int sm_count();  // capi.cu
+
 }  // namespace w4a8
 
 using namespace w4a8;
@@ -107,28 +472,37 @@ W4A8_API w4a8_status w4a8_attn_weights(const void* q, int32_t q_row_stride, cons
         return set_error(W4A8_EINVAL, "%s: q row stride %d (a multiple of 8 that holds the heads)", what, q_row_stride);
     if (max_q < 0 || max_q > (1 << 24) || max_kv < 0 || acc_stride < max_kv)
         return set_error(W4A8_EINVAL, "%s: max_q=%d max_kv=%d, %d weights a head", what, max_q, max_kv, acc_stride);
-    if (!(scale == scale) || scale < 0.f) return set_error(W4A8_EINVAL, "%s: scale %g", what, scale);
+    if (!(scale > 0.f) || scale > 1e30f) return set_error(W4A8_EINVAL, "%s: scale %g", what, scale);
     if (tokens == 0 || max_q == 0 || max_kv == 0) return W4A8_OK;
-    p.q = q;
-    p.q_row = q_row_stride;
     p.H = H;
     p.KVH = KVH;
-    p.D = D;
+    p.G = H / KVH;
+    p.nch = (D + 63) / 64;
+    p.tpt = kTile / p.G;
+    p.box_tokens = max_q < p.tpt ? max_q : p.tpt;
+    p.cols = (p.box_tokens * p.G + 15) / 16 * 16;
     p.scale = scale;
     p.lse = lse;
     p.acc = acc;
     p.acc_stride = acc_stride;
     p.max_q = max_q;
-    const size_t smem = static_cast<size_t>((kRows + kKeys) * (D + 1) + kRows * 33) * 4;
-    const dim3 grid((static_cast<unsigned>(max_kv) + kKeys - 1) / kKeys, KVH, batch);
-    static FuncAttr a16, ab16;
+    p.box_rows = cache_box_rows(page);
+    p.err = device_error_word();
+    CUtensorMap mq, mk;
+    st = encode_queries(&mq, q, dtype, H, D, q_row_stride, tokens, p.G, p.box_tokens, what);
+    if (st == W4A8_OK) st = encode_cache(&mk, &p.order, k, p.c, KVH, D, what);
+    if (st != W4A8_OK) return st;
+    const long long most = static_cast<long long>((max_kv + kTile - 1) / kTile) * KVH * batch;
+    const int grid = static_cast<int>(most < sm_count() ? most : sm_count());
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
+    static FuncAttr a16, ab16;
     if (dtype == W4A8_F16) {
-        st = ensure_smem(weights_rows_kernel<__half>, a16, smem, -1, what);
-        return st != W4A8_OK ? st : launch_pdl(what, weights_rows_kernel<__half>, grid, dim3(kThreads), smem, cs, p);
+        st = ensure_smem(weights_tc_kernel<__half>, a16, kSmemBytes, -1, what);
+        return st != W4A8_OK ? st : launch_pdl(what, weights_tc_kernel<__half>, dim3(grid), dim3(kThreads), kSmemBytes, cs, mq, mk, p);
     }
-    st = ensure_smem(weights_rows_kernel<__nv_bfloat16>, ab16, smem, -1, what);
-    return st != W4A8_OK ? st : launch_pdl(what, weights_rows_kernel<__nv_bfloat16>, grid, dim3(kThreads), smem, cs, p);
+    st = ensure_smem(weights_tc_kernel<__nv_bfloat16>, ab16, kSmemBytes, -1, what);
+    return st != W4A8_OK ? st
+                         : launch_pdl(what, weights_tc_kernel<__nv_bfloat16>, dim3(grid), dim3(kThreads), kSmemBytes, cs, mq, mk, p);
 }
 
 }  // extern "C"

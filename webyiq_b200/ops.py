@@ -379,9 +379,9 @@ def qk_norm_rope_kv(qkv, kv, batch, pos, rope, H, q_norm=None, k_norm=None, eps=
 
 
 def attn_paged_workspace(batch, tokens, H, KVH, D, device):
-    """Workspace of attn_paged for calls of this size (uint8, zeros; each call leaves its counters zero)."""
+    """Workspace of attn_paged for calls of this size (uint8; any contents)."""
     n = _lib.load().w4a8_attn_paged_workspace_bytes(tokens, H, KVH, D, batch.B, batch.max_q, batch.max_kv)
-    return torch.zeros(max(n, 256), dtype=torch.uint8, device=device)
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def attn_paged(q, kv, batch, scale=None, gate=None, o=None, lse=None, workspace=None):

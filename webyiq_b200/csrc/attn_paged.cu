@@ -14,15 +14,18 @@
 //    into tensor memory over S as 16-bit pairs, O += P V with P as the MMA's A operand.
 //    K tiles are K-major operands and V tiles MN-major ones straight from the page
 //    layout: nothing is transposed.
-//  - One thread owns a row (a tensor memory lane): maximum and sum need no shuffles.
+//  - Two threads share a row (a tensor memory lane), 64 of a step's scores each: maximum
+//    and sum need no shuffles, only an exchange of the two maxima through shared
+//    memory. (One thread a row left a scheduler two warps, which the exponentials' issue
+//    held up: 530 us against XXX for 2048 tokens over 16384 slots, 32 / 8 heads of 128.)
 //    The exponentials are taken against a reference that follows the maximum only when
 //    it has grown by more than 2^8, so O is rarely rescaled; P <= 2^8 keeps its relative
 //    precision, and f32 sums divide the reference out at the end.
 //  - P is rounded to the cache's type (the tensor core wants A and B alike): a relative
 //    error of 2^-11 (f16) or 2^-8 (bf16) a weight, of the size of the output's own
 //    rounding.  Its sum is taken before that rounding.
-//  - NQ = 2: two row tiles share each K and V tile, a softmax warpgroup each (head sizes
-//    up to 128).  NQ = 1: one row tile and one softmax warpgroup, two S buffers so
+//  - NQ = 2: two row tiles share each K and V tile, two softmax warpgroups each (head sizes
+//    up to 128).  NQ = 1: one row tile and two softmax warpgroups, two S buffers so
 //    that the next scores are computed meanwhile (256-wide heads, whose O takes
 //    half of tensor memory, and calls of up to 128 rows a kv head).
 //  - Two threads issue MMAs, each for its own S buffer (units of one parity): a thread
@@ -53,8 +56,9 @@ constexpr int kTile = 128;                  // rows of a query tile, and slots o
 constexpr uint32_t kChunkBytes = kTile * 128;  // 128 rows x 64 elements
 constexpr int kSegs = 4;
 constexpr int kMaxStages = 12;
-constexpr uint32_t kMiscBytes = 2048;
+constexpr uint32_t kMiscBytes = 3072;
 constexpr int kItemCost = 2;  // an item's start and end (query load, epilogue), in kv steps
+constexpr int kHalf = kTile / 2;  // scores of a row that one thread takes
 constexpr float kLazy = 8.0f;  // log2 of how far the maximum may pass its reference
 
 struct AttnParams {
@@ -95,20 +99,22 @@ struct Plan {
     static constexpr int kParts = NCH / kCps;        // stages of a K or V tile
     static constexpr uint32_t kStageBytes = kCps * kChunkBytes;
     static constexpr uint32_t kQBytes = NQ * NCH * kChunkBytes;
-    static constexpr int kFit = static_cast<int>((227 * 1024 - 1024 - kMiscBytes - kQBytes) / kStageBytes);
+    static constexpr int kFit = static_cast<int>((227 * 1024 - kMiscBytes - kQBytes) / kStageBytes);
     static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
-    static constexpr size_t kSmem = 1024 + kQBytes + kStages * kStageBytes + kMiscBytes;
-    static constexpr int kSoftWarps = 4 * NQ;
+    static constexpr size_t kSmem = kQBytes + kStages * kStageBytes + kMiscBytes;
+    static constexpr int kSoftWarps = 8;
     static constexpr int kThreads = (kSoftWarps + 4) * 32;
     static_assert(kStages >= 2 * kParts + (kParts == 1 ? 1 : 0), "ring too short");
 };
 
 struct Bars {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t s_full[2], p_full[2], o_done[2];
+    uint64_t s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][parity of the unit]
     uint64_t q_full, q_empty;
     uint64_t seg_full[kSegs], seg_empty[kSegs];
+    uint64_t pair[4];  // [quarter]: the two warps that share its rows (NQ = 1)
     Segment seg[kSegs];
+    float xch[2][2][kTile];  // [turn][half][row]
     uint32_t tmem;
     int abort;
 };
@@ -279,8 +285,12 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
     attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const AttnParams p) {
     using P = Plan<NCH, NQ>;
-    extern __shared__ unsigned char smem_raw[];
-    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    // the swizzled tiles want 1024-byte alignment, which dynamic shared memory has where there is no static
+    extern __shared__ __align__(1024) unsigned char smem[];
+    if (smem_u32(smem) & 1023) {
+        if (threadIdx.x == 0) atomicOr(p.err, DEV_ERR_ATTN_TIMEOUT);
+        return;
+    }
     unsigned char* ring = smem + P::kQBytes;
     Bars& bars = *reinterpret_cast<Bars*>(ring + P::kStages * P::kStageBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -291,10 +301,11 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
             mbar_init(&bars.full[s], 1);
             mbar_init(&bars.empty[s], 2);  // both MMA warps, whether they use the tile or not
         }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&bars.s_full[i], 1);
-            mbar_init(&bars.p_full[i], 4);
-            mbar_init(&bars.o_done[i], 1);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&bars.s_full[0][i], 1);
+            mbar_init(&bars.p_full[0][i], NQ == 2 ? 4 : 8);
+            mbar_init(&bars.o_done[0][i], 1);
+            mbar_init(&bars.pair[i], 2);
         }
         mbar_init(&bars.q_full, 1);
         mbar_init(&bars.q_empty, 2);
@@ -329,8 +340,6 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
         return s.j1 > 0;
     };
 
-    // NQ = 2: 384 threads of 168 registers; 256 x 200 + 128 x 104 is their sum
-    if (NQ == 2 && warp >= P::kSoftWarps) setmaxnreg_dec<104>();
     if (warp == kLineWarp) {
         // ---- the work line: this CTA's stretch of it, segment by segment ----
         // kv steps of sequence b0 + lane, all its kv heads
@@ -552,9 +561,9 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
         if (qs > 0) mbar_wait(&bars.q_full, (qs - 1) & 1);
     } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
         // ---- MMA: S(u) = Q K(u)^T once P of this buffer's previous unit has been used by O += P V ----
-        const int w = warp - kMmaWarp;  // S buffer, and row tile where there are two
-        constexpr uint32_t id_qk = idesc_f16<T>(kTile, false), id_pv = idesc_f16<T>(P::kCps * 64, true);
-        const uint32_t s_tm = tmem + w * 128;
+        const int w = warp - kMmaWarp;  // row tile (NQ = 2), or the parity of its units (NQ = 1)
+        constexpr uint32_t id_qk = idesc_f16<T>(NQ == 2 ? kHalf : kTile, false), id_pv = idesc_f16<T>(P::kCps * 64, true);
+        const uint32_t s_tm = tmem + w * kTile;
         const uint32_t o_tm = tmem + kO + (NQ == 2 ? w * NCH * 64 : 0);
         const uint32_t q_sm = smem_u32(smem) + (NQ == 2 ? w * NCH * kChunkBytes : 0);
         bool ok = true;
@@ -576,107 +585,189 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                 for (int part = 0; part < P::kParts; ++part) mbar_arrive(&bars.empty[(pos + part) % P::kStages]);
             __syncwarp();
         };
-        auto own = [&](uint32_t u) { return NQ == 2 || (u & 1) == static_cast<uint32_t>(w); };
-        // O += P(u) V; valid < 128 where the V tile reaches past the sequence
-        auto pv = [&](uint32_t u, bool first, int valid) {
-            const uint32_t pos = (NQ == 2 ? 2 * u + 1 : 2 * u + 2) * P::kParts;
-            if (!own(u)) return tile_skip(pos);
-            if (!tile_wait(pos)) return;
-            if (valid < kTile) {
-                // clear the rows of slots past the length (NQ = 2: both warps, the same zeros)
-                for (int part = 0; part < P::kParts; ++part) {
-                    unsigned char* v = ring + ((pos + part) % P::kStages) * P::kStageBytes;
-                    for (int e = valid * 8 + lane; e < kTile * 8; e += 32)
-#pragma unroll
-                        for (int ch = 0; ch < P::kCps; ++ch)
-                            *reinterpret_cast<uint4*>(v + ch * kChunkBytes + e * 16) = make_uint4(0, 0, 0, 0);
-                }
-                fence_proxy_async();
-                __syncwarp();
-            }
-            if (!wait(&bars.p_full[w], (NQ == 2 ? u : u >> 1) & 1)) return;
-            // one O: the units take turns, each after the one before
-            if (NQ == 1 && u > 0 && !wait(&bars.o_done[w ^ 1], ((u - 1) >> 1) & 1)) return;
-            tc1_fence_after();
-            if (lane == 0) {
-#pragma unroll
-                for (int part = 0; part < P::kParts; ++part) {
-                    const uint32_t st = (pos + part) % P::kStages;
-                    const uint32_t v = smem_u32(ring + st * P::kStageBytes);
-#pragma unroll
-                    for (int kk = 0; kk < kTile / 16; ++kk)
-                        mma_f16_ts(o_tm + part * P::kCps * 64, s_tm + kk * 8, desc_mn_major(v + kk * 2048, kChunkBytes),
-                                   id_pv, !first || kk > 0);
-                    tc1_commit(&bars.empty[st]);
-                }
-                tc1_commit(&bars.o_done[w]);
-            }
-            __syncwarp();
-        };
-        // S(u) = Q K^T; fresh: the segment's Q has not been waited for
-        auto qk = [&](uint32_t u, bool& fresh, uint32_t seg) {
-            const uint32_t pos = (NQ == 2 ? 2 * u : (u == 0 ? 0 : 2 * u - 1)) * P::kParts;
-            if (!own(u)) return tile_skip(pos);
-            if (fresh && !wait(&bars.q_full, seg & 1)) return;
-            fresh = false;
+        auto v_pos = [&](uint32_t u) { return (NQ == 2 ? 2 * u + 1 : 2 * u + 2) * P::kParts; };
+        auto k_pos = [&](uint32_t u) { return (NQ == 2 ? 2 * u : (u == 0 ? 0 : 2 * u - 1)) * P::kParts; };
+        // clears the rows of slots past the sequence in V tile u (NQ = 2: both warps, the same zeros)
+        auto clear = [&](uint32_t u, int valid) {
+            if (valid >= kTile) return;
             for (int part = 0; part < P::kParts; ++part) {
-                if (!wait(&bars.full[(pos + part) % P::kStages], ((pos + part) / P::kStages) & 1)) return;
-                tc1_fence_after();
-                if (lane == 0) {
-                    const uint32_t st = (pos + part) % P::kStages;
-                    const uint32_t k = smem_u32(ring + st * P::kStageBytes);
+                unsigned char* v = ring + ((v_pos(u) + part) % P::kStages) * P::kStageBytes;
+                for (int e = valid * 8 + lane; e < kTile * 8; e += 32)
 #pragma unroll
                     for (int ch = 0; ch < P::kCps; ++ch)
-#pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            mma_f16_ss(s_tm, desc_k_major(q_sm + (part * P::kCps + ch) * kChunkBytes + kk * 32),
-                                       desc_k_major(k + ch * kChunkBytes + kk * 32), id_qk, part + ch + kk > 0);
-                    tc1_commit(&bars.empty[st]);
-                }
-                __syncwarp();
+                        *reinterpret_cast<uint4*>(v + ch * kChunkBytes + e * 16) = make_uint4(0, 0, 0, 0);
             }
-            if (lane == 0) tc1_commit(&bars.s_full[w]);
+            fence_proxy_async();
             __syncwarp();
         };
-        uint32_t u = 0, segs = 0;
-        bool have = false, first = false;  // the unit before u: its P V is due
-        int valid = kTile;
-        Segment g;
-        while (ok && next_seg(g)) {
-            bool fresh = true;
-            for (int j = g.j0; j < g.j1 && ok; ++j, ++u) {
-                // in the ring's order: NQ = 2: V(u - 1) K(u), NQ = 1: K(u) V(u - 1)
-                if (NQ == 2 && have) pv(u - 1, first, valid);
-                if (ok) qk(u, fresh, segs);
-                if (NQ == 1 && have && ok) pv(u - 1, first, valid);
-                have = true;
-                first = j == g.j0;
-                valid = max(min(g.len - j * kTile, kTile), 0);
+        // One thread's MMAs, back to back: a barrier test or a commit between them would hold the
+        // tensor core up by 200 or 60 clocks.  Unit x is a kv step (NQ = 1), or half of one: the
+        // weights and the V rows from 64 * half on.
+        auto pv_mma = [&](uint32_t u, int half, bool first) {
+            constexpr int kSteps = (NQ == 2 ? kHalf : kTile) / 16;
+            const uint32_t p_tm = s_tm + half * kHalf;
+#pragma unroll
+            for (int part = 0; part < P::kParts; ++part) {
+                const uint32_t v = smem_u32(ring + ((v_pos(u) + part) % P::kStages) * P::kStageBytes) + half * kHalf * 128;
+#pragma unroll
+                for (int kk = 0; kk < kSteps; ++kk)
+                    mma_f16_ts(o_tm + part * P::kCps * 64, p_tm + kk * 8, desc_mn_major(v + kk * 2048, kChunkBytes), id_pv,
+                               !first || kk > 0);
             }
-            // through with the segment's Q: a warp that had no unit in it comes after its load all the same,
-            // or its arrival could count for the segment before
-            if (ok && fresh) wait(&bars.q_full, segs & 1);
-            if (!ok) break;
-            if (lane == 0) tc1_commit(&bars.q_empty);
-            __syncwarp();
-            ++segs;
+        };
+        auto qk_mma = [&](uint32_t u, int half) {
+#pragma unroll
+            for (int part = 0; part < P::kParts; ++part) {
+                const uint32_t k = smem_u32(ring + ((k_pos(u) + part) % P::kStages) * P::kStageBytes) + half * kHalf * 128;
+#pragma unroll
+                for (int ch = 0; ch < P::kCps; ++ch)
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        mma_f16_ss(s_tm + half * kHalf, desc_k_major(q_sm + (part * P::kCps + ch) * kChunkBytes + kk * 32),
+                                   desc_k_major(k + ch * kChunkBytes + kk * 32), id_qk, part + ch + kk > 0);
+            }
+        };
+        auto release = [&](uint32_t pos) {
+            for (int part = 0; part < P::kParts; ++part) tc1_commit(&bars.empty[(pos + part) % P::kStages]);
+        };
+        uint32_t u = 0, segs = 0;
+        Segment g;
+        if (NQ == 2) {
+            // S of half step x once the weights of half step x - 2, which lie in its place, have been used
+            bool first[2] = {false, false};  // [half] of the step before: its first P V overwrites O
+            int valid = kTile;
+            auto pv = [&](uint32_t x) {
+                const uint32_t v = x >> 1;
+                const int half = static_cast<int>(x & 1);
+                if (half == 0) {
+                    if (!tile_wait(v_pos(v))) return false;
+                    clear(v, valid);
+                }
+                if (!wait(&bars.p_full[w][half], v & 1)) return false;
+                tc1_fence_after();
+                if (lane == 0) pv_mma(v, half, first[half]);
+                return true;
+            };
+            auto pv_done = [&](uint32_t x) {
+                tc1_commit(&bars.o_done[w][x & 1]);
+                if (x & 1) release(v_pos(x >> 1));
+            };
+            while (ok && next_seg(g)) {
+                for (int j = g.j0; j < g.j1 && ok; ++j, ++u) {
+                    for (int half = 0; half < 2 && ok; ++half) {
+                        const uint32_t x = 2 * u + half;
+                        if (u > 0 && !pv(x - 2)) break;
+                        if (half == 0 && ((j == g.j0 && !wait(&bars.q_full, segs & 1)) || !tile_wait(k_pos(u)))) break;
+                        tc1_fence_after();
+                        if (lane == 0) {
+                            qk_mma(u, half);
+                            tc1_commit(&bars.s_full[w][half]);
+                            if (u > 0) pv_done(x - 2);
+                            if (half) release(k_pos(u));
+                        }
+                        __syncwarp();
+                    }
+                    first[0] = j == g.j0;
+                    valid = max(min(g.len - j * kTile, kTile), 0);
+                }
+                if (!ok) break;
+                if (lane == 0) tc1_commit(&bars.q_empty);  // through with the segment's Q
+                __syncwarp();
+                ++segs;
+            }
+            for (uint32_t x = 2 * u - 2; ok && u > 0 && x < 2 * u; ++x) {
+                if (pv(x) && lane == 0) pv_done(x);
+                __syncwarp();
+            }
+        } else {
+            // S(u) once P(u - 2) has been used; the units of one parity are this warp's
+            auto own = [&](uint32_t x) { return (x & 1) == static_cast<uint32_t>(w); };
+            auto pv = [&](uint32_t x, bool first, int valid) {
+                if (!own(x)) return tile_skip(v_pos(x));
+                if (!tile_wait(v_pos(x))) return;
+                clear(x, valid);
+                if (!wait(&bars.p_full[0][w], (x >> 1) & 1)) return;
+                // one O: the units take turns, each after the one before
+                if (x > 0 && !wait(&bars.o_done[0][w ^ 1], ((x - 1) >> 1) & 1)) return;
+                tc1_fence_after();
+                if (lane == 0) {
+                    pv_mma(x, 0, first);
+                    tc1_commit(&bars.o_done[0][w]);
+                    release(v_pos(x));
+                }
+                __syncwarp();
+            };
+            bool have = false, first = false;  // the unit before u: its P V is due
+            int valid = kTile;
+            while (ok && next_seg(g)) {
+                bool fresh = true;  // the segment's Q has not been waited for
+                for (int j = g.j0; j < g.j1 && ok; ++j, ++u) {
+                    // in the ring's order: K(u) V(u - 1)
+                    if (!own(u)) {
+                        tile_skip(k_pos(u));
+                    } else if ((!fresh || wait(&bars.q_full, segs & 1)) && tile_wait(k_pos(u))) {
+                        fresh = false;
+                        tc1_fence_after();
+                        if (lane == 0) {
+                            qk_mma(u, 0);
+                            tc1_commit(&bars.s_full[0][w]);
+                            release(k_pos(u));
+                        }
+                        __syncwarp();
+                    }
+                    if (have && ok) pv(u - 1, first, valid);
+                    have = true;
+                    first = j == g.j0;
+                    valid = max(min(g.len - j * kTile, kTile), 0);
+                }
+                // through with the segment's Q: a warp that had no unit in it comes after its load all the
+                // same, or its arrival could count for the segment before
+                if (ok && fresh) wait(&bars.q_full, segs & 1);
+                if (!ok) break;
+                if (lane == 0) tc1_commit(&bars.q_empty);
+                __syncwarp();
+                ++segs;
+            }
+            if (ok && have) pv(u - 1, first, valid);
         }
-        if (ok && have) pv(u - 1, first, valid);
     } else {
         // ---- softmax, one thread a row, and the output ----
-        if (NQ == 2) setmaxnreg_inc<200>();
-        constexpr int kOut = NQ == 2 ? 32 : 64;  // columns of O in registers at a time
-        const int grp = NQ == 2 ? warp / 4 : 0;
-        const int r = (warp & 3) * 32 + lane;  // row of the tile
-        const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        // NQ = 2: a warpgroup a row tile, 64 slots a unit.  NQ = 1: two warpgroups, 64 of a unit's 128 slots each.
+        constexpr int kOut = 32;                              // columns of O in registers at a time
+        constexpr int kUnits = NQ == 2 ? 2 : 1;               // units of a kv step
+        const int grp = NQ == 2 ? warp >> 2 : 0, half = NQ == 2 ? 0 : warp >> 2, quarter = warp & 3;
+        const int r = quarter * 32 + lane;  // row of the tile
+        const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t o_tm = tmem + lane_off + kO + grp * NCH * 64;
         const float c = p.scale * 1.44269504088896340736f;
         const int tok_in = r / p.G, head_in = r - tok_in * p.G;
+        // this warp's columns of the output
+        const int mid = (p.D / 2 + 15) / 16 * 16;
+        const int d0 = half ? mid : 0, d1 = NQ == 2 || half ? p.D : mid;
         uint32_t u = 0;  // units so far of this group
         bool ok = true;
+        // The other warp of these rows: a meeting, and x for its x.
+        uint32_t turns = 0;
+        auto meet = [&]() {
+            tc1_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.pair[quarter]);
+            ok = !*bail.flag && bail.wait(&bars.pair[quarter], turns & 1);
+            ++turns;
+            ok = __all_sync(kFull, ok);
+            tc1_fence_after();
+            return ok;
+        };
+        auto swap = [&](float x, float& other) {
+            const int at = turns & 1;
+            bars.xch[at][half][r] = x;
+            if (!meet()) return false;
+            other = bars.xch[at][half ^ 1][r];
+            return true;
+        };
         // O after unit x of this group
         auto o_wait = [&](uint32_t x) {
-            ok = !*bail.flag && bail.wait(&bars.o_done[NQ == 2 ? grp : (x & 1)], (NQ == 2 ? x : x >> 1) & 1);
+            ok = !*bail.flag && bail.wait(&bars.o_done[grp][x & 1], (x >> 1) & 1);
             ok = __all_sync(kFull, ok);
             if (ok) tc1_fence_after();
             return ok;
@@ -696,47 +787,55 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                 // the gate is wanted at the segment's end: towards L2 now
                 const char* at = reinterpret_cast<const char*>(p.gate + static_cast<size_t>(t) * p.gate_row +
                                                                static_cast<size_t>(h) * p.gate_head);
-                for (int e = 0; e < p.D * 4; e += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + e));
+                for (int e = d0 * 4; e < d1 * 4; e += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + e));
             }
             float m = -INFINITY, l = 0.f;
-            for (int j = g.j0; j < g.j1 && ok; ++j, ++u) {
-                const uint32_t buf = NQ == 2 ? grp : (u & 1), use = NQ == 2 ? u : u >> 1;
-                ok = !*bail.flag && bail.wait(&bars.s_full[buf], use & 1);
+            for (int j = g.j0 * kUnits; j < g.j1 * kUnits && ok; ++j, ++u) {
+                ok = !*bail.flag && bail.wait(&bars.s_full[grp][u & 1], (u >> 1) & 1);
                 if (!__all_sync(kFull, ok)) {
                     ok = false;
                     break;
                 }
                 tc1_fence_after();
                 if (any_live) {
-                    const uint32_t s_tm = tmem + lane_off + buf * 128;
-                    float s[kTile];
+                    // scores and weights of this thread: 64 columns, and 32 at the start of the unit's place
+                    const uint32_t unit = tmem + lane_off + (NQ == 2 ? grp * kTile + (u & 1) * kHalf : (u & 1) * kTile);
+                    const uint32_t s_tm = unit + half * kHalf, p_tm = unit + half * (kHalf / 2);
+                    const int kv0 = NQ == 2 ? j * kHalf : j * kTile + half * kHalf;
+                    float s[kHalf];
+                    float mx = m;
 #pragma unroll
-                    for (int i = 0; i < kTile; i += 32) tmem1_ld32(s_tm + i, s + i);
+                    for (int q = 0; q < kHalf; q += 32) tmem1_ld32(s_tm + q, s + q);
                     tmem1_wait_ld();
-                    const int kv0 = j * kTile;
-                    if (kv0 + kTile - 1 > min(least, g.len - 1)) {
-                        const int lm = min(lim, g.len - 1) - kv0;
+                    if (kv0 + kHalf - 1 > min(least, g.len - 1)) {
+                        const int lm = min(lim, g.len - 1) - kv0;  // last column this row sees
 #pragma unroll
-                        for (int i = 0; i < kTile; ++i)
+                        for (int i = 0; i < kHalf; ++i)
                             if (i > lm) s[i] = -INFINITY;
                     }
-                    float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
+                    float y0 = s[0], y1 = s[1], y2 = s[2];
 #pragma unroll
-                    for (int i = 4; i < kTile; i += 4) {
-                        m0 = fmaxf(m0, s[i]);
-                        m1 = fmaxf(m1, s[i + 1]);
-                        m2 = fmaxf(m2, s[i + 2]);
-                        m3 = fmaxf(m3, s[i + 3]);
+                    for (int i = 0; i < kHalf; i += 8) {
+                        mx = max3(mx, s[i], s[i + 1]);
+                        y0 = max3(y0, s[i + 2], s[i + 3]);
+                        y1 = max3(y1, s[i + 4], s[i + 5]);
+                        y2 = max3(y2, s[i + 6], s[i + 7]);
                     }
-                    const float mx = fmaxf(fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)), m);
+                    mx = fmaxf(max3(mx, y0, y1), y2);
+                    if (NQ == 1) {
+                        // (the other warp has its scores, too, once this returns: its columns may be overwritten)
+                        float other;
+                        if (!swap(mx, other)) break;
+                        mx = fmaxf(mx, other);
+                    }
                     if (__any_sync(kFull, live && (mx - m) * c > kLazy)) {
                         const float f = mx == m ? 1.f : ex2((m - mx) * c);
                         m = mx;
                         l *= f;
-                        if (j > g.j0) {
+                        if (j > g.j0 * kUnits) {
                             if (!o_wait(u - 1)) break;
 #pragma unroll 1
-                            for (int i = 0; i < NCH * 64; i += 16) {
+                            for (int i = d0 / 16 * 16; i < (NQ == 2 || half ? NCH * 64 : mid); i += 16) {
                                 float o[16];
                                 tmem1_ld16(o_tm + i, o);
                                 tmem1_wait_ld();
@@ -749,73 +848,77 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                     const float neg = m == -INFINITY ? 0.f : -m * c;
                     const float2 c2 = make_float2(c, c), neg2 = make_float2(neg, neg);
                     float2 l0 = make_float2(0.f, 0.f), l1 = make_float2(0.f, 0.f);
+                    uint32_t w[kHalf / 2];
 #pragma unroll
-                    for (int h = 0; h < kTile; h += 64) {
-                        uint32_t w[32];
-#pragma unroll
-                        for (int i = 0; i < 64; i += 4) {
-                            float2 a = __ffma2_rn(make_float2(s[h + i], s[h + i + 1]), c2, neg2);
-                            float2 b = __ffma2_rn(make_float2(s[h + i + 2], s[h + i + 3]), c2, neg2);
-                            a.x = ex2(a.x);
-                            a.y = ex2(a.y);
-                            b.x = ex2(b.x);
-                            b.y = ex2(b.y);
-                            l0 = __fadd2_rn(l0, a);
-                            l1 = __fadd2_rn(l1, b);
-                            w[i / 2] = Elem<T>::pack(a.x, a.y);
-                            w[i / 2 + 1] = Elem<T>::pack(b.x, b.y);
-                        }
-                        tmem1_st32(s_tm + h / 2, w);
+                    for (int i = 0; i < kHalf; i += 4) {
+                        float2 a = __ffma2_rn(make_float2(s[i], s[i + 1]), c2, neg2);
+                        float2 b = __ffma2_rn(make_float2(s[i + 2], s[i + 3]), c2, neg2);
+                        a.x = ex2(a.x);
+                        a.y = ex2(a.y);
+                        b.x = ex2(b.x);
+                        b.y = ex2(b.y);
+                        l0 = __fadd2_rn(l0, a);
+                        l1 = __fadd2_rn(l1, b);
+                        w[i / 2] = Elem<T>::pack(a.x, a.y);
+                        w[i / 2 + 1] = Elem<T>::pack(b.x, b.y);
                     }
+                    tmem1_st32(p_tm, w);
                     l += (l0.x + l0.y) + (l1.x + l1.y);
                     tmem1_wait_st();
                     tc1_fence_before();
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.p_full[buf]);
+                if (lane == 0) mbar_arrive(&bars.p_full[grp][u & 1]);
             }
             if (!ok) break;
             if (!o_wait(u - 1)) break;
+            if (NQ == 1 && any_live) {
+                float other;
+                if (!swap(l, other) || !meet()) break;  // the second: both have read, the place may be written again
+                l += other;
+            }
             if (g.parts == 1) {
                 if (any_live) {
                     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
-                    for (int col = 0; col < p.D; col += kOut) {
+                    for (int col = d0; col < d1; col += kOut) {
                         // a chunk's gates are asked for at once: a load's latency a chunk, not a load
                         float o[kOut];
                         float4 gate[kOut / 4];
                         if (p.gate && live)
 #pragma unroll
                             for (int e = 0; e < kOut; e += 8)
-                                if (col + e < p.D) load_gate8(p, t, h, col + e, gate + e / 4);
+                                if (col + e < d1) load_gate8(p, t, h, col + e, gate + e / 4);
 #pragma unroll
-                        for (int e = 0; e < kOut; e += 32) tmem1_ld32(o_tm + col + e, o + e);
+                        for (int e = 0; e < kOut; e += 16) tmem1_ld16(o_tm + col + e, o + e);
                         tmem1_wait_ld();
                         if (live)
 #pragma unroll
                             for (int e = 0; e < kOut; e += 8)
-                                if (col + e < p.D) put8<T>(p, t, h, col + e, o + e, inv, gate + e / 4);
+                                if (col + e < d1) put8<T>(p, t, h, col + e, o + e, inv, gate + e / 4);
                         __syncwarp();
                     }
-                    if (live && p.lse) p.lse[static_cast<size_t>(t) * p.H + h] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
+                    if (live && half == 0 && p.lse)
+                        p.lse[static_cast<size_t>(t) * p.H + h] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
                 }
             } else if (any_live) {
                 // a shared item: this CTA's part (neighbouring rows' 16 bytes lie side by side)
                 const size_t sl = part_slot<NQ>(blockIdx.x, g.first, grp);
                 float4* dst = p.part + sl * (p.D / 4) * p.rows_cap + r;
 #pragma unroll 1
-                for (int col = 0; col < p.D; col += 32) {
-                    float o[32];
-                    tmem1_ld32(o_tm + col, o);
+                for (int col = d0; col < d1; col += kOut) {
+                    float o[kOut];
+#pragma unroll
+                    for (int e = 0; e < kOut; e += 16) tmem1_ld16(o_tm + col + e, o + e);
                     tmem1_wait_ld();
                     if (live) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            if (col + e < p.D) dst[static_cast<size_t>((col + e) / 4) * p.rows_cap] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        for (int e = 0; e < kOut; e += 4)
+                            if (col + e < d1) dst[static_cast<size_t>((col + e) / 4) * p.rows_cap] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                     }
                     __syncwarp();
                 }
-                if (live) p.ml[sl * p.rows_cap + r] = make_float2(m, l);
+                if (live && half == 0) p.ml[sl * p.rows_cap + r] = make_float2(m, l);
             }
             tc1_fence_before();
         }

@@ -134,14 +134,11 @@ __device__ __forceinline__ void tma_load_3d_at(uint32_t dst, const CUtensorMap* 
         : "memory");
 }
 
-// Registers of a warpgroup, from and to the block's share at launch.
-template <int N>
-__device__ __forceinline__ void setmaxnreg_inc() {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void setmaxnreg_dec() {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+// The largest of three (one instruction).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
 }
 
 __device__ __forceinline__ float ex2(float x) {

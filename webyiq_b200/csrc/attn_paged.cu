@@ -112,7 +112,8 @@ struct Bars {
     uint64_t s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][parity of the unit]
     uint64_t q_full, q_empty;
     uint64_t seg_full[kSegs], seg_empty[kSegs];
-    uint64_t pair[4];  // [quarter]: the two warps that share its rows (NQ = 1)
+    uint64_t pair[4];     // [quarter]: the two warps that share its rows (NQ = 1)
+    uint64_t turn[2][4];  // [row tile][quarter]: its exponentials' turn (NQ = 2)
     Segment seg[kSegs];
     float xch[2][2][kTile];  // [turn][half][row]
     uint32_t tmem;
@@ -306,6 +307,8 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
             mbar_init(&bars.p_full[0][i], NQ == 2 ? 4 : 8);
             mbar_init(&bars.o_done[0][i], 1);
             mbar_init(&bars.pair[i], 2);
+            mbar_init(&bars.turn[0][i], 1);
+            mbar_init(&bars.turn[1][i], 1);
         }
         mbar_init(&bars.q_full, 1);
         mbar_init(&bars.q_empty, 2);
@@ -797,7 +800,20 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                     break;
                 }
                 tc1_fence_after();
-                if (any_live) {
+                // The two row tiles' warps of one scheduler take turns at the exponentials: side by side
+                // both would take twice as long and then leave the unit idle together.
+                auto take_turn = [&]() {
+                    if (NQ == 1 || (grp == 0 && u == 0)) return true;
+                    ok = !*bail.flag && bail.wait(&bars.turn[grp][quarter], (grp == 0 ? u - 1 : u) & 1);
+                    return ok = __all_sync(kFull, ok);
+                };
+                auto pass_turn = [&]() {
+                    if (NQ == 2 && lane == 0) mbar_arrive(&bars.turn[grp ^ 1][quarter]);
+                };
+                if (!any_live) {
+                    if (!take_turn()) break;
+                    pass_turn();
+                } else {
                     // scores and weights of this thread: 64 columns, and 32 at the start of the unit's place
                     const uint32_t unit = tmem + lane_off + (NQ == 2 ? grp * kTile + (u & 1) * kHalf : (u & 1) * kTile);
                     const uint32_t s_tm = unit + half * kHalf, p_tm = unit + half * (kHalf / 2);
@@ -848,6 +864,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                     const float neg = m == -INFINITY ? 0.f : -m * c;
                     const float2 c2 = make_float2(c, c), neg2 = make_float2(neg, neg);
                     float2 l0 = make_float2(0.f, 0.f), l1 = make_float2(0.f, 0.f);
+                    if (!take_turn()) break;
                     uint32_t w[kHalf / 2];
 #pragma unroll
                     for (int i = 0; i < kHalf; i += 4) {
@@ -862,6 +879,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                         w[i / 2] = Elem<T>::pack(a.x, a.y);
                         w[i / 2 + 1] = Elem<T>::pack(b.x, b.y);
                     }
+                    pass_turn();
                     tmem1_st32(p_tm, w);
                     l += (l0.x + l0.y) + (l1.x + l1.y);
                     tmem1_wait_st();

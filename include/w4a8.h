@@ -341,7 +341,8 @@ enum { W4A8_F16 = 0, W4A8_BF16 = 1, W4A8_F32 = 2 };
  * past the table take its last row): (a, b) -> (a cos - b sin, b cos + a sin) for the
  * pairs (i, i + rot / 2), or (2i, 2i + 1) with interleaved.  q_out [tokens, H, D] of the
  * cache's type; key and value of token i of n go to slot kv_len - n + i (nowhere where
- * that is negative).  Values past f16's range become its largest value. */
+ * that is negative).  Values past f16's range become its largest value.  qkv, q_out,
+ * the norm weights and rope are 16-byte aligned. */
 W4A8_API w4a8_status w4a8_qk_norm_rope_kv(const float* qkv, int32_t qkv_row_stride, int32_t q_head_stride, int32_t H,
                                           int32_t KVH, int32_t D, const float* q_norm, const float* k_norm, float eps,
                                           const float* rope, int32_t rot, int32_t rope_rows, int32_t interleaved,

@@ -372,6 +372,12 @@ def test_evict(cuda, KVH, D, page, lens, keep, kind, dtype):
     np.testing.assert_array_equal(c.host(c.k), rk)
 
 
+def test_evict_past_shared_memory(cuda):
+    """More slots than a CTA keeps the keys of in shared memory, ties among them."""
+    test_evict(cuda, 1, 80, 16, [60000, 52000], [20011, 51999], "ties", "f16")
+    test_evict(cuda, 1, 80, 16, [60000, 51201], [59990, 7], "spread", "bf16")
+
+
 def test_bad_indices_stay_in_range(cuda):
     """Lengths, starts and pages out of range are bounded by the kernels: values of no meaning, no
     access out of range, the context stays usable."""

@@ -267,16 +267,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t q_bytes = static_cast<uint32_t>(p.box_tokens) * p.G * 128;
         uint32_t kn = 0, qn = 0;
         bool ok = true;
-        Item it;
-        while (ok && next_item(it)) {
+        // page and row of this lane's box of an item: looked up an item ahead
+        auto locate = [&](const Item& it, int& page, int& row, int& n) {
             const int s0 = it.j * kTile + lane * p.box_rows;
-            const int n = min(boxes, (it.len - it.j * kTile + p.box_rows - 1) / p.box_rows);
-            int page = 0, row = 0;
+            n = min(boxes, (it.len - it.j * kTile + p.box_rows - 1) / p.box_rows);
+            page = row = 0;
             if (lane < n) {
                 const int pi = s0 / p.c.page;
                 page = static_cast<int>(page_of(p.b, p.c, it.seq, pi));
                 row = s0 - pi * p.c.page;
             }
+        };
+        Item it, next;
+        int page = 0, row = 0, n = 0, page_next = 0, row_next = 0, n_next = 0;
+        bool more = next_item(it);
+        if (more) locate(it, page, row, n);
+        for (; ok && more; it = next, page = page_next, row = row_next, n = n_next) {
+            more = next_item(next);
+            if (more) locate(next, page_next, row_next, n_next);
             for (int ch = 0; ch < p.nch && ok; ++ch, ++kn) {
                 const uint32_t st = kn % kKRing;
                 ok = !*bail.flag && bail.wait(&sm.k_empty[st], ((kn / kKRing) & 1) ^ 1);
@@ -348,63 +356,79 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int tok_in = gt / p.G, head_in = gt - tok_in * p.G;  // this thread's column when offsets are fetched
         uint32_t sn = 0, turn = 0, done = 0;
         bool ok = true;
-        Item it;
-        while (ok && next_item(it)) {
+        // this thread's column's offset in row tile i of an item: asked for a tile ahead
+        auto offset = [&](const Item& it, int i) {
+            const int tok = (it.i0 + i) * p.tpt + tok_in;
+            if (i >= it.steps || tok_in >= p.tpt || tok >= it.n) return 0.f;
+            return ld_dep(p.lse + static_cast<size_t>(it.t0 + tok) * p.H + it.kh * p.G + head_in);
+        };
+        // the first row tile of an item that is this group's, if the item's first is number s of all
+        auto first = [&](uint32_t s) { return static_cast<int>((s ^ static_cast<uint32_t>(grp)) & 1); };
+        Item it, next;
+        bool more = next_item(it);
+        float pre = more ? offset(it, first(sn)) : 0.f;
+        while (more && ok) {
+            more = next_item(next);
+            const int i_first = first(sn), i_next = first(sn + it.steps);
+            const float pre_next = more ? offset(next, i_next) : 0.f;
             const int slot = it.j * kTile + gt;
             float total = 0.f;
-            for (int i = 0; i < it.steps && ok; ++i, ++sn) {
-                if (static_cast<int>(sn & 1) != grp) continue;
+            for (int i = i_first; i < it.steps && ok; i += 2) {
                 const int tok0 = (it.i0 + i) * p.tpt;
                 const int toks = min(it.n - tok0, p.tpt);
                 // offsets of the tile's columns, for the whole group
                 float* off = sm.off[grp][turn & 1];
-                float mine = 0.f;
-                if (tok_in < toks)
-                    mine = ld_dep(p.lse + static_cast<size_t>(it.t0 + tok0 + tok_in) * p.H + it.kh * p.G + head_in) *
-                           -1.44269504088896340736f;
-                off[gt] = mine;
+                off[gt] = pre * -1.44269504088896340736f;
+                pre = offset(it, i + 2);
                 mbar_arrive(&sm.group[grp]);
                 ok = !*bail.flag && bail.wait(&sm.group[grp], turn & 1);
                 ++turn;
-                const uint32_t buf = sn % kSBufs;
-                ok = ok && !*bail.flag && bail.wait(&sm.s_full[buf], (sn / kSBufs) & 1);
+                const uint32_t buf = (sn + i) % kSBufs;
+                ok = ok && !*bail.flag && bail.wait(&sm.s_full[buf], ((sn + i) / kSBufs) & 1);
                 if (!(ok = __all_sync(kFull, ok))) break;
                 tc1_fence_after();
                 const uint32_t s_tm = tmem + lane_off + buf * kTile;
                 const int cols = toks * p.G;
                 // the first column that sees this slot
                 const int lo = max(slot - (it.vis + tok0), 0) * p.G;
-                // every slot of the warp is seen by every column, and every column is live
-                const bool all = __all_sync(kFull, lo == 0) && cols % 32 == 0;
                 float2 a0 = make_float2(0.f, 0.f), a1 = make_float2(0.f, 0.f);
-                for (int x = 0; x < cols; x += 32) {
-                    float s[32];
-                    if (x + 32 <= p.cols) {
-                        tmem1_ld32(s_tm + x, s);
-                    } else {  // 16 columns: the MMA wrote no more
-                        tmem1_ld16(s_tm + x, s);
-#pragma unroll
-                        for (int e = 16; e < 32; ++e) s[e] = 0.f;
+                auto add = [&](const float* s, int x, int e, bool masked) {
+                    const float4 o = *reinterpret_cast<const float4*>(off + x + e);
+                    float2 u = __ffma2_rn(make_float2(s[e], s[e + 1]), c2, make_float2(o.x, o.y));
+                    float2 v = __ffma2_rn(make_float2(s[e + 2], s[e + 3]), c2, make_float2(o.z, o.w));
+                    u.x = ex2(u.x);
+                    u.y = ex2(u.y);
+                    v.x = ex2(v.x);
+                    v.y = ex2(v.y);
+                    if (masked) {
+                        const int q = x + e;
+                        u.x = q >= lo && q < cols ? u.x : 0.f;
+                        u.y = q + 1 >= lo && q + 1 < cols ? u.y : 0.f;
+                        v.x = q + 2 >= lo && q + 2 < cols ? v.x : 0.f;
+                        v.y = q + 3 >= lo && q + 3 < cols ? v.y : 0.f;
                     }
-                    tmem1_wait_ld();
+                    a0 = __fadd2_rn(a0, u);
+                    a1 = __fadd2_rn(a1, v);
+                };
+                if (cols == kTile && __all_sync(kFull, lo == 0)) {
+                    // every column is live and sees every slot of the warp
+                    float s[kTile];
+                    tmem1_ld32(s_tm, s);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 o = *reinterpret_cast<const float4*>(off + x + e);
-                        float2 u = __ffma2_rn(make_float2(s[e], s[e + 1]), c2, make_float2(o.x, o.y));
-                        float2 v = __ffma2_rn(make_float2(s[e + 2], s[e + 3]), c2, make_float2(o.z, o.w));
-                        u.x = ex2(u.x);
-                        u.y = ex2(u.y);
-                        v.x = ex2(v.x);
-                        v.y = ex2(v.y);
-                        if (!all) {
-                            const int q = x + e;
-                            u.x = q >= lo && q < cols ? u.x : 0.f;
-                            u.y = q + 1 >= lo && q + 1 < cols ? u.y : 0.f;
-                            v.x = q + 2 >= lo && q + 2 < cols ? v.x : 0.f;
-                            v.y = q + 3 >= lo && q + 3 < cols ? v.y : 0.f;
-                        }
-                        a0 = __fadd2_rn(a0, u);
-                        a1 = __fadd2_rn(a1, v);
+                    for (int x = 0; x < kTile; x += 32) {
+                        tmem1_wait_ld();
+                        if (x + 32 < kTile) tmem1_ld32(s_tm + x + 32, s + x + 32);  // one load ahead
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) add(s + x, x, e, false);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int x = 0; x < cols; x += 16) {
+                        float s[16];
+                        tmem1_ld16(s_tm + x, s);
+                        tmem1_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) add(s, x, e, true);
                     }
                 }
                 total += (a0.x + a0.y) + (a1.x + a1.y);
@@ -413,21 +437,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (lane == 0) mbar_arrive(&sm.s_empty[buf]);
             }
             if (!ok) break;
-            // the second group hands its share of the item to the first
-            const uint32_t d = done & 1, phase = (done >> 1) & 1;
-            ++done;
-            ok = !*bail.flag && bail.wait(grp == 1 ? &sm.sum_empty[d] : &sm.sum_full[d], grp == 1 ? phase ^ 1 : phase);
-            if (!(ok = __all_sync(kFull, ok))) break;
-            if (grp == 1)
-                sm.sum[d][gt] = total;
-            else
-                total += sm.sum[d][gt];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(grp == 1 ? &sm.sum_full[d] : &sm.sum_empty[d]);
-            if (grp == 0 && slot < it.len) {
+            bool writes = i_first == 0;  // a single row tile: the group that has it
+            if (it.steps > 1) {
+                // the second group hands its share of the item to the first
+                const uint32_t d = done & 1, phase = (done >> 1) & 1;
+                ++done;
+                ok = !*bail.flag && bail.wait(grp == 1 ? &sm.sum_empty[d] : &sm.sum_full[d], grp == 1 ? phase ^ 1 : phase);
+                if (!(ok = __all_sync(kFull, ok))) break;
+                if (grp == 1)
+                    sm.sum[d][gt] = total;
+                else
+                    total += sm.sum[d][gt];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(grp == 1 ? &sm.sum_full[d] : &sm.sum_empty[d]);
+                writes = grp == 0;
+            }
+            if (writes && slot < it.len) {
                 float* at = p.acc + (static_cast<size_t>(it.seq) * p.KVH + it.kh) * p.acc_stride + slot;
                 *at = ld_dep(at) + total;
             }
+            sn += it.steps;
+            it = next;
+            pre = pre_next;
         }
     }
 

@@ -375,13 +375,18 @@ W4A8_API size_t w4a8_attn_paged_workspace_bytes(int32_t tokens, int32_t H, int32
 /* The attention weight each slot received from the batch's new tokens, added to acc
  * f32[batch, KVH, acc_stride] (acc_stride >= max_kv): acc[b, kvh, j] += the sum over
  * the new tokens that see slot j and the query heads of kvh of exp(scale q k_j - lse), with
- * q and lse as w4a8_attn_paged takes and gives them.  The same inputs give the same bits. */
+ * q and lse as w4a8_attn_paged takes and gives them.  The same inputs give the same bits.
+ * workspace: w4a8_attn_weights_workspace_bytes(...) bytes (of the current device; 0 where a
+ * kv head has at most 128 query rows, and workspace may be NULL), 16-byte aligned, any
+ * contents; calls that share one must not overlap on the GPU. */
 W4A8_API w4a8_status w4a8_attn_weights(const void* q, int32_t q_row_stride, const float* lse, int32_t H, int32_t KVH,
                                        int32_t D, float scale, const uint32_t* q_start, const uint32_t* kv_len,
                                        const uint32_t* table, int32_t batch, int32_t table_stride, int32_t tokens,
                                        int32_t max_q, int32_t max_kv, const void* k, int32_t dtype, int32_t pages,
                                        int32_t page, size_t page_stride, int32_t head_stride, int32_t row_stride,
-                                       float* acc, int32_t acc_stride, void* stream);
+                                       float* acc, int32_t acc_stride, void* workspace, size_t workspace_bytes,
+                                       void* stream);
+W4A8_API size_t w4a8_attn_weights_workspace_bytes(int32_t H, int32_t KVH, int32_t max_q);
 
 /* Eviction by accumulated weight, for each sequence and kv head on its own: of len =
  * kv_len[b] slots the n = min(len, keep[b]) stay that come first by (protected, weight

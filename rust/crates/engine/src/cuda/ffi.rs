@@ -129,8 +129,9 @@ extern "C" {
                              scale: f32, q_start: *const u32, kv_len: *const u32, table: *const u32, batch: i32,
                              table_stride: i32, tokens: i32, max_q: i32, max_kv: i32, k: *const c_void,
                              dtype: i32, pages: i32, page: i32, page_stride: usize, head_stride: i32,
-                             row_stride: i32, acc: *mut f32, acc_stride: i32,
-                             stream: *mut c_void) -> w4a8_status;
+                             row_stride: i32, acc: *mut f32, acc_stride: i32, workspace: *mut c_void,
+                             workspace_bytes: usize, stream: *mut c_void) -> w4a8_status;
+    pub fn w4a8_attn_weights_workspace_bytes(h: i32, kvh: i32, max_q: i32) -> usize;
     pub fn w4a8_kv_evict(k: *mut c_void, v: *mut c_void, dtype: i32, pages: i32, page: i32, page_stride: usize,
                          head_stride: i32, row_stride: i32, kvh: i32, d: i32, kv_len: *const u32,
                          table: *const u32, batch: i32, table_stride: i32, acc: *const f32, pos: *const u32,

@@ -38,11 +38,11 @@ def _attn(**kw):
 
 
 def _weights(**kw):
-    a = _args(**{**dict(q=256, qrow=8 * 128, lse=256, acc=256, stride=100), **kw})
+    a = _args(**{**dict(q=256, qrow=8 * 128, lse=256, acc=256, stride=100, ws=0, wsn=0), **kw})
     return _lib.load().w4a8_attn_weights(
         P(a["q"]), a["qrow"], P(a["lse"]), a["H"], a["KVH"], a["D"], a["scale"], P(a["q_start"]), P(a["kv_len"]),
         P(a["table"]), a["batch"], a["per"], a["tokens"], a["max_q"], a["max_kv"], P(a["k"]), a["dtype"], a["pages"],
-        a["page"], a["ps"], a["hs"], a["rs"], P(a["acc"]), a["stride"], None)
+        a["page"], a["ps"], a["hs"], a["rs"], P(a["acc"]), a["stride"], P(a["ws"]), a["wsn"], None)
 
 
 def _evict(**kw):
@@ -70,7 +70,7 @@ STEP = [dict(q_start=0), dict(tokens=-1), dict(tokens=1 << 25), dict(H=7), dict(
                              dict(gate=256, gr=4, gh=-4), dict(max_q=-1), dict(max_kv=-1), dict(scale=math.nan),
                              dict(scale=-1.0), dict(ws=0), dict(wsn=0), dict(ws=260)]),
     (_weights, SHARED + STEP + [dict(q=0), dict(lse=0), dict(acc=0), dict(q=264), dict(acc=258), dict(qrow=1000),
-                                dict(stride=99), dict(max_q=-1), dict(scale=math.nan)]),
+                                dict(stride=99), dict(max_q=-1), dict(scale=math.nan), dict(max_q=40), dict(max_q=40, ws=264, wsn=1 << 20)]),
     (_evict, SHARED + [dict(v=0), dict(acc=0), dict(pos=0), dict(keep=0), dict(low=0), dict(acc_out=0), dict(pos_out=0),
                        dict(len_out=0), dict(len_out=512), dict(stride=0), dict(sink=-1), dict(ws=0), dict(wsn=0),
                        dict(batch=40000), dict(ws=260)])])
@@ -103,6 +103,7 @@ def test_workspace_sizes():
     L = _lib.load()
     assert L.w4a8_kv_evict_workspace_bytes(0, 1, 1) == 0
     assert L.w4a8_kv_evict_workspace_bytes(4, 8, 30016) >= 4 * 8 * 30016 // 2 * 8
+    assert L.w4a8_attn_weights_workspace_bytes(8, 2, 32) == 0 < L.w4a8_attn_weights_workspace_bytes(8, 2, 33)
     assert L.w4a8_attn_paged_workspace_bytes(1, 8, 2, 256, 1, 1, 100000) >= 16
 
 

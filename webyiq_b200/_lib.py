@@ -66,7 +66,8 @@ _SIGS = {
                                        ctypes.c_size_t, _P]),
     "w4a8_attn_paged_workspace_bytes": (ctypes.c_size_t, [_I, _I, _I, _I, _I, _I, _I]),
     "w4a8_attn_weights": (ctypes.c_int, [_P, _I, _P, _I, _I, _I, ctypes.c_float, _P, _P, _P, _I, _I, _I, _I, _I, _P,
-                                         _I, _I, _I, ctypes.c_size_t, _I, _I, _P, _I, _P]),
+                                         _I, _I, _I, ctypes.c_size_t, _I, _I, _P, _I, _P, ctypes.c_size_t, _P]),
+    "w4a8_attn_weights_workspace_bytes": (ctypes.c_size_t, [_I, _I, _I]),
     "w4a8_kv_evict": (ctypes.c_int, [_P, _P, _I, _I, _I, ctypes.c_size_t, _I, _I, _I, _I, _P, _P, _I, _I, _P, _P,
                                      _I, _P, _P, _I, _P, _P, _P, _P, ctypes.c_size_t, _P]),
     "w4a8_kv_evict_workspace_bytes": (ctypes.c_size_t, [_I, _I, _I]),

@@ -11,14 +11,18 @@
 // column, read from shared memory (one broadcast load for four).
 //
 // An item is one tile of slots of a kv head; it stays in shared memory while the query
-// rows that see it pass.  Items lie on a line weighted by their row tiles (plus one for
-// the tile itself), and each CTA takes those that start in an equal stretch of it, found
-// on the device from the batch's lengths.  Single tokens are bound by HBM (K is read
-// once), chunks by the exponentials: 128 x 128 of them take the SM's 16 a clock 1024
-// clocks, the MMA half of that at 128-wide heads.
+// rows that see it pass.  Items lie on a line, each as long as its row tiles and one for
+// the tile itself, and each CTA takes an equal stretch of it, found on the device from
+// the batch's lengths.  An item that a stretch boundary cuts leaves its parts' sums in the
+// workspace, and a small kernel adds those in the order of the stretches.  Single tokens
+// are bound by HBM (K is read once), chunks by the exponentials: 128 x 128 of them take
+// the SM's 16 a clock 1024 clocks, the MMA half of that at 128-wide heads.
 //
-// Warp roles: two softmax warpgroups that take row tiles in turn (four S buffers, so
-// the MMAs run ahead), then TMA, MMA, and the warp that walks the line.
+// Warp roles: four softmax warpgroups that take row tiles in turn, an S buffer each, so
+// that one's waits and loads run beside the others' exponentials (two left the unit idle
+// half of the time), then TMA, MMA, and the warp that walks the line.
+#include <algorithm>
+
 #include "launch.cuh"
 #include "tc_f16.cuh"
 
@@ -28,21 +32,26 @@ namespace {
 
 constexpr int kTile = 128;
 constexpr uint32_t kChunkBytes = kTile * 128;  // 128 rows x 64 elements
-constexpr int kKRing = 7, kQRing = 6;          // 16 KB chunks of slots and of query rows
-constexpr int kSBufs = 4, kItems = 4;
-constexpr int kSoftWarps = 8, kThreads = (kSoftWarps + 4) * 32;
+constexpr int kRing = 13 * kChunkBytes;         // tiles of slots, then tiles of query rows
+constexpr int kMaxStages = 8;
+constexpr int kGroups = 4, kItems = 4;
+constexpr int kSoftWarps = 4 * kGroups, kThreads = (kSoftWarps + 4) * 32;
 
 struct WeightParams {
     int H, KVH, G, nch;
     int tpt;         // tokens of a row tile
     int box_tokens;  // tokens that one load of query rows brings
     int cols;        // N of the MMA: box_tokens * G rounded up to 16
+    uint32_t k_stages, q_stages;
+    uint32_t k_bytes, q_bytes;  // of a tile in the ring
     float scale;
     const float* lse;
     float* acc;
     int acc_stride, max_q;
     int box_rows;
     CacheOrder order;
+    int4* shared_items;  // [CTA] the item that starts in its stretch and goes on in the next: row, tile, slots, parts
+    float* part;         // [CTA][2][128]
     unsigned int* err;
     PagedCache c;
     PagedBatch b;
@@ -53,18 +62,18 @@ struct Item {
     int t0, n;      // the sequence's first new token (global) and how many
     int vis;        // last slot its first new token sees
     int len, j;     // slots, and the tile's number
-    int i0, steps;  // first row tile that sees the tile's first slot, and how many from it; steps == 0: the end
+    int i0, steps;  // row tiles, of those that see something of the slots; steps == 0: the end
+    int first, parts;  // first CTA of the item, CTAs that share it
 };
 
 struct Smem {
-    unsigned char k[kKRing][kChunkBytes];
-    unsigned char q[kQRing][kChunkBytes];
-    float off[2][2][kTile];  // [group][turn][column]: -lse * log2 e
-    float sum[2][kTile];     // the second group's sums of an item, on the way to the first
-    uint64_t k_full[kKRing], k_empty[kKRing], q_full[kQRing], q_empty[kQRing];
-    uint64_t s_full[kSBufs], s_empty[kSBufs];
+    unsigned char ring[kRing];
+    float off[kGroups][2][kTile];      // [group][turn][column]: -lse * log2 e
+    float sum[2][kGroups - 1][kTile];  // [turn]: the other groups' sums of an item, on the way to the first
+    uint64_t k_full[kMaxStages], k_empty[kMaxStages], q_full[kMaxStages], q_empty[kMaxStages];
+    uint64_t s_full[kGroups], s_empty[kGroups];
     uint64_t item_full[kItems], item_empty[kItems];
-    uint64_t group[2], sum_full[2], sum_empty[2];
+    uint64_t group[kGroups], sum_full[2], sum_empty[2];
     Item item[kItems];
     uint32_t tmem;
     int abort;
@@ -77,6 +86,24 @@ __device__ __forceinline__ int first_row_tile(const SeqSpan& s, int j, int tpt) 
     return max(0, j * kTile - (s.len - s.n)) / tpt;
 }
 
+// A CTA's part of the item that starts in its stretch lies second, of the one that came over first.
+__device__ __forceinline__ size_t part_at(int cta, int first) {
+    return (static_cast<size_t>(cta) * 2 + (cta == first ? 1 : 0)) * kTile;
+}
+
+__global__ void __launch_bounds__(kTile) weights_merge_kernel(const WeightParams p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int first = blockIdx.x;
+    const int4 item = ld_dep(p.shared_items + first);
+    const int slot = item.y * kTile + threadIdx.x;
+    if (item.w == 0 || slot >= item.z) return;
+    float total = 0.f;
+    for (int q = 0; q < item.w; ++q) total += ld_dep(p.part + part_at(first + q, first) + threadIdx.x);
+    float* at = p.acc + static_cast<size_t>(item.x) * p.acc_stride + slot;
+    *at = ld_dep(at) + total;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     weights_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -84,28 +111,26 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ unsigned char smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int kTmaWarp = kSoftWarps, kMmaWarp = kTmaWarp + 1, kLineWarp = kTmaWarp + 2;
+    constexpr int kTmaWarp = kSoftWarps, kMmaWarp = kTmaWarp + 1, kLineWarp = kTmaWarp + 3;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kKRing; ++i) {
+        for (int i = 0; i < kMaxStages; ++i) {
             mbar_init(&sm.k_full[i], 1);
-            mbar_init(&sm.k_empty[i], 1);
-        }
-        for (int i = 0; i < kQRing; ++i) {
+            mbar_init(&sm.k_empty[i], 2);  // both MMA warps, whether they use the tile or not
             mbar_init(&sm.q_full[i], 1);
-            mbar_init(&sm.q_empty[i], 1);
+            mbar_init(&sm.q_empty[i], 2);
         }
-        for (int i = 0; i < kSBufs; ++i) {
+        for (int i = 0; i < kGroups; ++i) {
             mbar_init(&sm.s_full[i], 1);
             mbar_init(&sm.s_empty[i], 4);
+            mbar_init(&sm.group[i], 128);
         }
         for (int i = 0; i < kItems; ++i) {
             mbar_init(&sm.item_full[i], 1);
-            mbar_init(&sm.item_empty[i], kSoftWarps + 2);
+            mbar_init(&sm.item_empty[i], kSoftWarps + 3);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sm.group[i], 128);
-            mbar_init(&sm.sum_full[i], 4);
+            mbar_init(&sm.sum_full[i], kSoftWarps - 4);
             mbar_init(&sm.sum_empty[i], 4);
         }
         sm.abort = 0;
@@ -172,7 +197,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int off = 16; off > 0; off >>= 1) mine += __shfl_xor_sync(kFull, mine, off);
             total += mine;
         }
-        const long long at = blockIdx.x * total / gridDim.x, end = (blockIdx.x + 1) * total / gridDim.x;
+        const long long ctas = min(static_cast<long long>(gridDim.x), total), me = blockIdx.x;
+        long long at = 0, end = 0;
+        if (me < ctas) {
+            at = me * total / ctas;
+            end = (me + 1) * total / ctas;
+        }
+        // the CTA whose stretch holds place x
+        auto cta_of = [&](long long x) { return static_cast<int>(((x + 1) * ctas - 1) / total); };
         int seq = 0, kh = 0, j = 0;
         long long pos = 0;  // start of item (seq, kh, j)
         bool ok = true;
@@ -199,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 pos += __shfl_sync(kFull, upto, 31);
             }
             span(seq, s, n, tiles);
-            // the first item that starts at `at` or past it
+            // the item that holds place `at`
             for (int j0 = 0; j0 < tiles; j0 += 32) {
                 const int len = j0 + lane < tiles ? item_len(s, n, j0 + lane) : 0;
                 int upto = len;
@@ -208,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int y = __shfl_up_sync(kFull, upto, off);
                     if (lane >= off) upto += y;
                 }
-                const unsigned past = __ballot_sync(kFull, j0 + lane < tiles && pos + upto - len >= at);
+                const unsigned past = __ballot_sync(kFull, pos + upto > at);
                 if (past) {
                     const int f = __ffs(past) - 1;
                     j = j0 + f;
@@ -231,7 +263,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             ++sent;
             return true;
         };
-        while (ok && at < end) {
+        int4 shared_item = make_int4(0, 0, 0, 0);
+        while (ok && pos < end) {
             if (j >= tiles) {  // the next kv head or sequence
                 j = 0;
                 if (++kh == p.KVH) {
@@ -243,7 +276,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (seq >= p.b.batch) break;
                 }
             }
-            if (pos >= end) break;
             Item it;
             it.seq = seq;
             it.kh = kh;
@@ -252,19 +284,30 @@ __global__ void __launch_bounds__(kThreads, 1)
             it.vis = s.len - s.n;
             it.len = min(s.len, p.acc_stride);
             it.j = j;
-            it.i0 = first_row_tile(s, j, p.tpt);
-            it.steps = (n + p.tpt - 1) / p.tpt - it.i0;
-            if (it.steps > 0) publish(it);
-            pos += max(it.steps, 0) + 1;
+            const int i0 = first_row_tile(s, j, p.tpt), steps = max((n + p.tpt - 1) / p.tpt - i0, 0);
+            const long long start = pos + 1;
+            const int lo = static_cast<int>(max(at - start, 0ll)), hi = static_cast<int>(min(static_cast<long long>(steps), end - start));
+            it.i0 = i0 + lo;
+            it.steps = hi - lo;
+            if (hi > lo) {
+                it.first = cta_of(start);
+                it.parts = cta_of(start + steps - 1) - it.first + 1;
+                if (it.parts > 1 && it.first == static_cast<int>(blockIdx.x))
+                    shared_item = make_int4(seq * p.KVH + kh, j, it.len, it.parts);
+                if (!publish(it)) break;
+            }
+            pos += steps + 1;
+            at = pos;
             ++j;
         }
+        if (lane == 0 && p.shared_items) p.shared_items[blockIdx.x] = shared_item;
         Item stop{};
         if (ok) publish(stop);
     } else if (warp == kTmaWarp) {
         // ---- TMA: the item's slots, then the query rows, chunk by chunk ----
         const int boxes = kTile / p.box_rows;
         const uint32_t box_bytes = static_cast<uint32_t>(p.box_rows) * 128;
-        const uint32_t q_bytes = static_cast<uint32_t>(p.box_tokens) * p.G * 128;
+        const uint32_t q_load = static_cast<uint32_t>(p.box_tokens) * p.G * 128;  // a chunk's bytes
         uint32_t kn = 0, qn = 0;
         bool ok = true;
         // page and row of this lane's box of an item: looked up an item ahead
@@ -285,36 +328,39 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (; ok && more; it = next, page = page_next, row = row_next, n = n_next) {
             more = next_item(next);
             if (more) locate(next, page_next, row_next, n_next);
-            for (int ch = 0; ch < p.nch && ok; ++ch, ++kn) {
-                const uint32_t st = kn % kKRing;
-                ok = !*bail.flag && bail.wait(&sm.k_empty[st], ((kn / kKRing) & 1) ^ 1);
+            const uint32_t ks = kn % p.k_stages;
+            ok = !*bail.flag && bail.wait(&sm.k_empty[ks], ((kn / p.k_stages) & 1) ^ 1);
+            if (!(ok = __all_sync(kFull, ok))) break;
+            if (lane == 0) mbar_expect_tx(&sm.k_full[ks], static_cast<uint32_t>(n) * box_bytes * p.nch);
+            __syncwarp();
+            if (lane < n)
+                for (int ch = 0; ch < p.nch; ++ch)
+                    tma_load_4d(smem_u32(sm.ring) + ks * p.k_bytes + ch * kChunkBytes + lane * box_bytes, &tm_k, ch * 64,
+                                p.order.pick(0, row, it.kh, page), p.order.pick(1, row, it.kh, page),
+                                p.order.pick(2, row, it.kh, page), &sm.k_full[ks]);
+            ++kn;
+            for (int i = it.i0; i < it.i0 + it.steps; ++i, ++qn) {
+                const uint32_t qs = qn % p.q_stages;
+                ok = !*bail.flag && bail.wait(&sm.q_empty[qs], ((qn / p.q_stages) & 1) ^ 1);
                 if (!(ok = __all_sync(kFull, ok))) break;
-                if (lane == 0) mbar_expect_tx(&sm.k_full[st], static_cast<uint32_t>(n) * box_bytes);
+                if (lane == 0) mbar_expect_tx(&sm.q_full[qs], q_load * p.nch);
                 __syncwarp();
-                if (lane < n)
-                    tma_load_4d(smem_u32(sm.k[st]) + lane * box_bytes, &tm_k, ch * 64, p.order.pick(0, row, it.kh, page),
-                                p.order.pick(1, row, it.kh, page), p.order.pick(2, row, it.kh, page), &sm.k_full[st]);
-            }
-            for (int i = it.i0; i < it.i0 + it.steps && ok; ++i) {
-                for (int ch = 0; ch < p.nch && ok; ++ch, ++qn) {
-                    const uint32_t st = qn % kQRing;
-                    ok = !*bail.flag && bail.wait(&sm.q_empty[st], ((qn / kQRing) & 1) ^ 1);
-                    if (!(ok = __all_sync(kFull, ok))) break;
-                    if (lane == 0) {
-                        mbar_expect_tx(&sm.q_full[st], q_bytes);
-                        tma_load_3d_at(smem_u32(sm.q[st]), &tm_q, ch * 64, it.kh * p.G, it.t0 + i * p.tpt, &sm.q_full[st]);
-                    }
-                    __syncwarp();
-                }
+                if (lane < p.nch)
+                    tma_load_3d_at(smem_u32(sm.ring) + p.k_stages * p.k_bytes + qs * p.q_bytes + lane * (p.q_bytes / p.nch), &tm_q,
+                                   lane * 64, it.kh * p.G, it.t0 + i * p.tpt, &sm.q_full[qs]);
             }
         }
         // no copy may still be landing when the CTA exits
-        for (uint32_t x = kn > kKRing ? kn - kKRing : 0; x < kn; ++x) mbar_wait(&sm.k_full[x % kKRing], (x / kKRing) & 1);
-        for (uint32_t x = qn > kQRing ? qn - kQRing : 0; x < qn; ++x) mbar_wait(&sm.q_full[x % kQRing], (x / kQRing) & 1);
-    } else if (warp == kMmaWarp) {
-        // ---- MMA: S^T = K Q^T per row tile ----
+        for (uint32_t x = kn > p.k_stages ? kn - p.k_stages : 0; x < kn; ++x)
+            mbar_wait(&sm.k_full[x % p.k_stages], (x / p.k_stages) & 1);
+        for (uint32_t x = qn > p.q_stages ? qn - p.q_stages : 0; x < qn; ++x)
+            mbar_wait(&sm.q_full[x % p.q_stages], (x / p.q_stages) & 1);
+    } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+        // ---- MMA: S^T = K Q^T, the even row tiles from one warp and the odd ones from the other (a barrier
+        //      test or a commit holds up its own thread's MMAs only).  Both follow every fill in order. ----
+        const uint32_t w = static_cast<uint32_t>(warp - kMmaWarp);
         const uint32_t idesc = idesc_f16<T>(0, false) | (static_cast<uint32_t>(p.cols >> 3) << 17);
-        uint32_t kn = 0, qn = 0, sn = 0;
+        uint32_t kn = 0, sn = 0;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
             ok = ok && !*bail.flag && bail.wait(bar, parity);
@@ -322,30 +368,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         Item it;
         while (ok && next_item(it)) {
-            for (int i = 0; i < it.steps && ok; ++i, ++sn) {
-                const uint32_t buf = sn % kSBufs;
-                if (!wait(&sm.s_empty[buf], ((sn / kSBufs) & 1) ^ 1)) break;
-                for (int ch = 0; ch < p.nch; ++ch) {
-                    const uint32_t ks = (kn + ch) % kKRing, qs = (qn + ch) % kQRing;
-                    if (i == 0 && !wait(&sm.k_full[ks], ((kn + ch) / kKRing) & 1)) break;
-                    if (!wait(&sm.q_full[qs], ((qn + ch) / kQRing) & 1)) break;
-                    tc1_fence_after();
-                    if (lane == 0) {
-                        const uint32_t ka = smem_u32(sm.k[ks]), qa = smem_u32(sm.q[qs]);
+            const uint32_t ks = kn % p.k_stages;
+            if (!wait(&sm.k_full[ks], (kn / p.k_stages) & 1)) break;
+            const uint32_t ka = smem_u32(sm.ring) + ks * p.k_bytes;
+            for (int i = 0; i < it.steps; ++i, ++sn) {
+                const uint32_t qs = sn % p.q_stages, buf = sn % kGroups;
+                if (!wait(&sm.q_full[qs], (sn / p.q_stages) & 1)) break;
+                if ((sn & 1) != w) {
+                    if (lane == 0) mbar_arrive(&sm.q_empty[qs]);
+                    __syncwarp();
+                    continue;
+                }
+                if (!wait(&sm.s_empty[buf], ((sn / kGroups) & 1) ^ 1)) break;
+                tc1_fence_after();
+                if (lane == 0) {
+                    const uint32_t qa = smem_u32(sm.ring) + p.k_stages * p.k_bytes + qs * p.q_bytes, qc = p.q_bytes / p.nch;
+                    for (int ch = 0; ch < p.nch; ++ch)
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            mma_f16_ss(tmem + buf * kTile, desc_k_major(ka + kk * 32), desc_k_major(qa + kk * 32), idesc,
-                                       ch + kk > 0);
-                        tc1_commit(&sm.q_empty[qs]);
-                        if (i == it.steps - 1) tc1_commit(&sm.k_empty[ks]);
-                    }
-                    __syncwarp();
+                            mma_f16_ss(tmem + buf * kTile, desc_k_major(ka + ch * kChunkBytes + kk * 32),
+                                       desc_k_major(qa + ch * qc + kk * 32), idesc, ch + kk > 0);
+                    tc1_commit(&sm.s_full[buf]);
+                    tc1_commit(&sm.q_empty[qs]);
                 }
-                if (lane == 0) tc1_commit(&sm.s_full[buf]);
                 __syncwarp();
-                qn += p.nch;
             }
-            kn += p.nch;
+            if (lane == 0 && ok) tc1_commit(&sm.k_empty[ks]);
+            __syncwarp();
+            ++kn;
         }
     } else if (warp < kSoftWarps) {
         // ---- exponentials and sums, one thread a slot ----
@@ -363,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             return ld_dep(p.lse + static_cast<size_t>(it.t0 + tok) * p.H + it.kh * p.G + head_in);
         };
         // the first row tile of an item that is this group's, if the item's first is number s of all
-        auto first = [&](uint32_t s) { return static_cast<int>((s ^ static_cast<uint32_t>(grp)) & 1); };
+        auto first = [&](uint32_t s) { return static_cast<int>((static_cast<uint32_t>(grp) - s) % kGroups); };
         Item it, next;
         bool more = next_item(it);
         float pre = more ? offset(it, first(sn)) : 0.f;
@@ -373,21 +423,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float pre_next = more ? offset(next, i_next) : 0.f;
             const int slot = it.j * kTile + gt;
             float total = 0.f;
-            for (int i = i_first; i < it.steps && ok; i += 2) {
+            for (int i = i_first; i < it.steps && ok; i += kGroups) {
                 const int tok0 = (it.i0 + i) * p.tpt;
                 const int toks = min(it.n - tok0, p.tpt);
                 // offsets of the tile's columns, for the whole group
                 float* off = sm.off[grp][turn & 1];
                 off[gt] = pre * -1.44269504088896340736f;
-                pre = offset(it, i + 2);
+                pre = offset(it, i + kGroups);
                 mbar_arrive(&sm.group[grp]);
                 ok = !*bail.flag && bail.wait(&sm.group[grp], turn & 1);
                 ++turn;
-                const uint32_t buf = (sn + i) % kSBufs;
-                ok = ok && !*bail.flag && bail.wait(&sm.s_full[buf], ((sn + i) / kSBufs) & 1);
+                ok = ok && !*bail.flag && bail.wait(&sm.s_full[grp], ((sn + i) / kGroups) & 1);
                 if (!(ok = __all_sync(kFull, ok))) break;
                 tc1_fence_after();
-                const uint32_t s_tm = tmem + lane_off + buf * kTile;
+                const uint32_t s_tm = tmem + lane_off + grp * kTile;
                 const int cols = toks * p.G;
                 // the first column that sees this slot
                 const int lo = max(slot - (it.vis + tok0), 0) * p.G;
@@ -412,14 +461,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 };
                 if (cols == kTile && __all_sync(kFull, lo == 0)) {
                     // every column is live and sees every slot of the warp
-                    float s[kTile];
-                    tmem1_ld32(s_tm, s);
-#pragma unroll
+#pragma unroll 1
                     for (int x = 0; x < kTile; x += 32) {
+                        float s[32];
+                        tmem1_ld32(s_tm + x, s);
                         tmem1_wait_ld();
-                        if (x + 32 < kTile) tmem1_ld32(s_tm + x + 32, s + x + 32);  // one load ahead
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) add(s + x, x, e, false);
+                        for (int e = 0; e < 32; e += 4) add(s, x, e, false);
                     }
                 } else {
 #pragma unroll 1
@@ -434,27 +482,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                 total += (a0.x + a0.y) + (a1.x + a1.y);
                 tc1_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.s_empty[buf]);
+                if (lane == 0) mbar_arrive(&sm.s_empty[grp]);
             }
             if (!ok) break;
             bool writes = i_first == 0;  // a single row tile: the group that has it
             if (it.steps > 1) {
-                // the second group hands its share of the item to the first
+                // the other groups hand their shares of the item to the first
                 const uint32_t d = done & 1, phase = (done >> 1) & 1;
                 ++done;
-                ok = !*bail.flag && bail.wait(grp == 1 ? &sm.sum_empty[d] : &sm.sum_full[d], grp == 1 ? phase ^ 1 : phase);
+                ok = !*bail.flag && bail.wait(grp ? &sm.sum_empty[d] : &sm.sum_full[d], grp ? phase ^ 1 : phase);
                 if (!(ok = __all_sync(kFull, ok))) break;
-                if (grp == 1)
-                    sm.sum[d][gt] = total;
+                if (grp)
+                    sm.sum[d][grp - 1][gt] = total;
                 else
-                    total += sm.sum[d][gt];
+#pragma unroll
+                    for (int x = 0; x < kGroups - 1; ++x) total += sm.sum[d][x][gt];
                 __syncwarp();
-                if (lane == 0) mbar_arrive(grp == 1 ? &sm.sum_full[d] : &sm.sum_empty[d]);
+                if (lane == 0) mbar_arrive(grp ? &sm.sum_full[d] : &sm.sum_empty[d]);
                 writes = grp == 0;
             }
-            if (writes && slot < it.len) {
-                float* at = p.acc + (static_cast<size_t>(it.seq) * p.KVH + it.kh) * p.acc_stride + slot;
-                *at = ld_dep(at) + total;
+            if (writes) {
+                if (it.parts > 1) {
+                    p.part[part_at(blockIdx.x, it.first) + gt] = total;
+                } else if (slot < it.len) {
+                    float* at = p.acc + (static_cast<size_t>(it.seq) * p.KVH + it.kh) * p.acc_stride + slot;
+                    *at = ld_dep(at) + total;
+                }
             }
             sn += it.steps;
             it = next;
@@ -480,12 +533,19 @@ using namespace w4a8;
 
 extern "C" {
 
+W4A8_API size_t w4a8_attn_weights_workspace_bytes(int32_t H, int32_t KVH, int32_t max_q) {
+    // a row tile takes all the query rows of a kv head: no item is cut
+    if (H < 1 || KVH < 1 || static_cast<long long>(H / KVH) * max_q <= kTile) return 0;
+    return static_cast<size_t>(sm_count()) * (sizeof(int4) + 2 * kTile * sizeof(float));
+}
+
 W4A8_API w4a8_status w4a8_attn_weights(const void* q, int32_t q_row_stride, const float* lse, int32_t H, int32_t KVH,
                                        int32_t D, float scale, const uint32_t* q_start, const uint32_t* kv_len,
                                        const uint32_t* table, int32_t batch, int32_t table_stride, int32_t tokens,
                                        int32_t max_q, int32_t max_kv, const void* k, int32_t dtype, int32_t pages,
                                        int32_t page, size_t page_stride, int32_t head_stride, int32_t row_stride,
-                                       float* acc, int32_t acc_stride, void* stream) {
+                                       float* acc, int32_t acc_stride, void* workspace, size_t workspace_bytes,
+                                       void* stream) {
     const char* what = "w4a8_attn_weights";
     WeightParams p{};
     p.c = PagedCache{const_cast<void*>(k), const_cast<void*>(k), dtype, pages, page, page_stride, head_stride, row_stride};
@@ -512,6 +572,11 @@ W4A8_API w4a8_status w4a8_attn_weights(const void* q, int32_t q_row_stride, cons
     p.tpt = kTile / p.G;
     p.box_tokens = max_q < p.tpt ? max_q : p.tpt;
     p.cols = (p.box_tokens * p.G + 15) / 16 * 16;
+    // the ring: two to four tiles of query rows (all they can use where they are few), slots in the rest
+    p.k_bytes = p.nch * kChunkBytes;
+    p.q_bytes = p.nch * p.cols * 128;
+    p.q_stages = std::min<uint32_t>(4, std::max<uint32_t>(2, kRing / 2 / p.q_bytes));
+    p.k_stages = std::min<uint32_t>(kMaxStages, (kRing - p.q_stages * p.q_bytes) / p.k_bytes);
     p.scale = scale;
     p.lse = lse;
     p.acc = acc;
@@ -519,21 +584,32 @@ W4A8_API w4a8_status w4a8_attn_weights(const void* q, int32_t q_row_stride, cons
     p.max_q = max_q;
     p.box_rows = cache_box_rows(page);
     p.err = device_error_word();
+    const size_t need = w4a8_attn_weights_workspace_bytes(H, KVH, max_q);
+    if (need && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
+        return set_error(W4A8_EINVAL, "%s: workspace NULL, misaligned or under %zu bytes", what, need);
+    p.shared_items = need ? static_cast<int4*>(workspace) : nullptr;
+    p.part = need ? reinterpret_cast<float*>(p.shared_items + sm_count()) : nullptr;
     CUtensorMap mq, mk;
     st = encode_queries(&mq, q, dtype, H, D, q_row_stride, tokens, p.G, p.box_tokens, what);
     if (st == W4A8_OK) st = encode_cache(&mk, &p.order, k, p.c, KVH, D, what);
     if (st != W4A8_OK) return st;
-    const long long most = static_cast<long long>((max_kv + kTile - 1) / kTile) * KVH * batch;
-    const int grid = static_cast<int>(most < sm_count() ? most : sm_count());
+    // as many CTAs as the line can have places
+    const long long tiles = (static_cast<long long>(max_kv) + kTile - 1) / kTile;
+    const long long rows = (static_cast<long long>(max_q) + p.tpt - 1) / p.tpt;
+    const long long most = std::min(tiles * (need ? rows + 1 : 1), 1ll << 20) * KVH * batch;
+    const int grid = static_cast<int>(std::min<long long>(most, sm_count()));
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
     static FuncAttr a16, ab16;
     if (dtype == W4A8_F16) {
         st = ensure_smem(weights_tc_kernel<__half>, a16, kSmemBytes, -1, what);
-        return st != W4A8_OK ? st : launch_pdl(what, weights_tc_kernel<__half>, dim3(grid), dim3(kThreads), kSmemBytes, cs, mq, mk, p);
+        if (st == W4A8_OK) st = launch_pdl(what, weights_tc_kernel<__half>, dim3(grid), dim3(kThreads), kSmemBytes, cs, mq, mk, p);
+    } else {
+        st = ensure_smem(weights_tc_kernel<__nv_bfloat16>, ab16, kSmemBytes, -1, what);
+        if (st == W4A8_OK)
+            st = launch_pdl(what, weights_tc_kernel<__nv_bfloat16>, dim3(grid), dim3(kThreads), kSmemBytes, cs, mq, mk, p);
     }
-    st = ensure_smem(weights_tc_kernel<__nv_bfloat16>, ab16, kSmemBytes, -1, what);
-    return st != W4A8_OK ? st
-                         : launch_pdl(what, weights_tc_kernel<__nv_bfloat16>, dim3(grid), dim3(kThreads), kSmemBytes, cs, mq, mk, p);
+    if (st != W4A8_OK || !need || grid == 1) return st;
+    return launch_pdl(what, weights_merge_kernel, dim3(grid), dim3(kTile), 0, cs, p);
 }
 
 }  // extern "C"

@@ -414,20 +414,29 @@ def attn_paged(q, kv, batch, scale=None, gate=None, o=None, lse=None, workspace=
     return o, lse
 
 
-def attn_weights(q, lse, kv, batch, acc, scale=None):
+def attn_weights_workspace(batch, H, KVH, device):
+    """Workspace of attn_weights for calls of this size (uint8; any contents), or None where none is needed."""
+    n = _lib.load().w4a8_attn_weights_workspace_bytes(H, KVH, batch.max_q)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def attn_weights(q, lse, kv, batch, acc, scale=None, workspace=None):
     """acc f32 [B, KVH, slots] += the attention weight each slot received from the new
     tokens (w4a8.h), with attn_paged's q, lse and scale.  Returns acc."""
     _need_rows("attn_weights: q", q, kv.dtype, kv.device)
     T, H, D = q.shape
-    _need_cuda(lse, acc)
+    _need_cuda(lse, acc, workspace)
     if D != kv.D or lse.numel() != T * H or lse.dtype != torch.float32:
         raise ValueError("attn_weights: q [tokens, H, D] of the cache's D, lse f32 [tokens, H]")
     if acc.dtype != torch.float32 or acc.dim() != 3 or acc.shape[:2] != (batch.B, kv.KVH):
         raise ValueError("attn_weights: acc f32 [B, KVH, slots]")
+    if workspace is None:
+        workspace = attn_weights_workspace(batch, H, kv.KVH, q.device)
     _lib.check(_lib.load().w4a8_attn_weights(
         _ptr(q), q.stride(0) if T > 1 else H * D, _ptr(lse), H, kv.KVH, D,
         1.0 / math.sqrt(D) if scale is None else scale, batch.pq, batch.pl, batch.pt, batch.B, batch.per, T,
-        batch.max_q, batch.max_kv, kv.pk, *kv.layout, _ptr(acc), acc.shape[2], _stream()))
+        batch.max_q, batch.max_kv, kv.pk, *kv.layout, _ptr(acc), acc.shape[2], _ptr(workspace),
+        0 if workspace is None else workspace.numel(), _stream()))
     return acc
 
 

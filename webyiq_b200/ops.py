@@ -312,8 +312,9 @@ class PagedKV:
         self.k, self.v = k, v
         self.pages, self.KVH, self.page, self.D = k.shape
         self.dtype, self.device = k.dtype, k.device
+        self.scale = 1.0 / math.sqrt(self.D)  # of the scores, where a call gives none
         self.layout = (_TYPES[k.dtype], self.pages, self.page, k.stride(0), k.stride(1), k.stride(2))
-        self.pk, self.pv = _ptr(k), _ptr(v)
+        self.pk, self.pv = k.data_ptr(), v.data_ptr()
 
     def __repr__(self):
         return f"PagedKV(pages={self.pages}, KVH={self.KVH}, page={self.page}, D={self.D}, {self.dtype})"
@@ -335,14 +336,42 @@ class PagedBatch:
         self.q_start, self.kv_len, self.table = q_start, kv_len, table
         self.max_q, self.max_kv = int(max_q), int(max_kv)
         self.per = table.shape[1]
-        self.pq, self.pl, self.pt = _ptr(q_start), _ptr(kv_len), _ptr(table)
+        self.pq, self.pl, self.pt = q_start.data_ptr(), kv_len.data_ptr(), table.data_ptr()
 
 
-def _need_rows(name, t, dtype, device):
-    """A [tokens, heads, D] tensor whose tokens may lie apart: (head, D) contiguous."""
-    if t.dtype != dtype or t.device != device or t.dim() != 3 or \
-            (t.numel() and (t.stride(2) != 1 or (t.stride(1) != t.shape[2] and t.shape[1] > 1))):
-        raise ValueError(f"{name}: a [tokens, heads, D] tensor of {dtype} on {device}, contiguous within a token")
+# The paged operators are called once a layer and token, so their wrappers keep to cheap
+# checks: each attribute of a tensor costs about a tenth of a microsecond.
+
+
+def _raw_stream(device):
+    """The current stream of a device as an integer (torch.cuda.current_stream builds an object: 3 us)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _is(t, dtype):
+    return t.dtype is dtype and t.is_cuda and t.is_contiguous()
+
+
+def _opt(t, dtype, what):
+    """Pointer of an optional contiguous CUDA tensor (0 for None)."""
+    if t is None:
+        return 0
+    if not _is(t, dtype):
+        raise ValueError(f"{what}: a contiguous CUDA tensor of {dtype}")
+    return t.data_ptr()
+
+
+def _token_stride(name, t, kv):
+    """Elements from token to token of a [tokens, heads, D] tensor of the cache's type, contiguous within a token."""
+    if t.dtype is not kv.dtype or t.device != kv.device or t.dim() != 3:
+        raise ValueError(f"{name}: a [tokens, heads, D] tensor of {kv.dtype} on {kv.device}")
+    T, H, D = t.shape
+    if D != kv.D:
+        raise ValueError(f"{name}: {D} dims, a cache of {kv.D}")
+    s = t.stride()
+    if T * H and (s[2] != 1 or (s[1] != D and H > 1)):
+        raise ValueError(f"{name}: contiguous within a token")
+    return s[0] if T > 1 else H * D
 
 
 def qk_norm_rope_kv(qkv, kv, batch, pos, rope, H, q_norm=None, k_norm=None, eps=1e-6, gated=False, interleaved=False,
@@ -352,29 +381,33 @@ def qk_norm_rope_kv(qkv, kv, batch, pos, rope, H, q_norm=None, k_norm=None, eps=
     heads of D in their place); pos int32 [tokens]; rope f32 [rows, rot] (cosines, then
     sines) or None; q_norm, k_norm f32 [D] or None.  Returns q [tokens, H, D] of the
     cache's type."""
-    _need_cuda(pos, rope, q_norm, k_norm, q)
-    if not qkv.is_cuda or qkv.dtype != torch.float32 or qkv.dim() != 2 or qkv.stride(1) != 1:
-        raise ValueError("qk_norm_rope_kv: qkv f32 [tokens, heads * D] with inner stride 1")
-    T, D = qkv.shape[0], kv.D
+    if qkv.dtype is not torch.float32 or qkv.device != kv.device or qkv.dim() != 2:
+        raise ValueError(f"qk_norm_rope_kv: qkv f32 [tokens, heads * D] on {kv.device}")
+    T, width = qkv.shape
+    D = kv.D
     qhs = 2 * D if gated else D
-    if qkv.shape[1] != H * qhs + 2 * kv.KVH * D:
-        raise ValueError(f"qk_norm_rope_kv: rows of {qkv.shape[1]} for {H} query and {kv.KVH} kv heads of {D}")
-    for w in (q_norm, k_norm):
-        if w is not None and (w.dtype != torch.float32 or w.numel() != D):
-            raise ValueError("qk_norm_rope_kv: norm weights f32 [D]")
-    rot = rows = 0
+    row, inner = qkv.stride()
+    if width != H * qhs + 2 * kv.KVH * D or (inner != 1 and T):
+        raise ValueError(f"qk_norm_rope_kv: rows of {width} for {H} query and {kv.KVH} kv heads of {D}, inner stride 1")
+    pqn, pkn = _opt(q_norm, torch.float32, "q_norm"), _opt(k_norm, torch.float32, "k_norm")
+    if (pqn and q_norm.numel() != D) or (pkn and k_norm.numel() != D):
+        raise ValueError("qk_norm_rope_kv: norm weights f32 [D]")
+    rot = rows = prope = ppos = 0
     if rope is not None:
-        if rope.dtype != torch.float32 or rope.dim() != 2 or pos is None or pos.dtype != torch.int32 or pos.numel() != T:
+        prope, ppos = _opt(rope, torch.float32, "rope"), _opt(pos, torch.int32, "pos")
+        if rope.dim() != 2 or not ppos and T or ppos and pos.numel() != T:
             raise ValueError("qk_norm_rope_kv: rope f32 [rows, rot] and pos int32 [tokens]")
         rows, rot = rope.shape
     if q is None:
         q = torch.empty((T, H, D), dtype=kv.dtype, device=qkv.device)
-    elif q.shape != (T, H, D) or q.dtype != kv.dtype:
-        raise ValueError("qk_norm_rope_kv: q [tokens, H, D] of the cache's type")
-    _lib.check(_lib.load().w4a8_qk_norm_rope_kv(
-        _ptr(qkv), qkv.stride(0) if T > 1 else qkv.shape[1], qhs, H, kv.KVH, D, _ptr(q_norm), _ptr(k_norm), eps,
-        _ptr(rope), rot, rows, interleaved, _ptr(pos), batch.pq, batch.pl, batch.pt, batch.B, batch.per, T, _ptr(q),
-        kv.pk, kv.pv, *kv.layout, _stream()))
+    elif q.shape != (T, H, D) or not _is(q, kv.dtype):
+        raise ValueError("qk_norm_rope_kv: q [tokens, H, D] of the cache's type, contiguous")
+    st = _lib.load().w4a8_qk_norm_rope_kv(
+        qkv.data_ptr(), row if T > 1 else width, qhs, H, kv.KVH, D, pqn, pkn, eps, prope, rot, rows, interleaved, ppos,
+        batch.pq, batch.pl, batch.pt, batch.B, batch.per, T, q.data_ptr(), kv.pk, kv.pv, *kv.layout,
+        _raw_stream(kv.device))
+    if st:
+        _lib.check(st)
     return q
 
 
@@ -389,28 +422,32 @@ def attn_paged(q, kv, batch, scale=None, gate=None, o=None, lse=None, workspace=
     type -> (o [tokens, H, D], lse f32 [tokens, H]); o of the cache's type, or f32 where
     an f32 o is given; gate f32 [tokens, H, D] (any token and head stride): o times
     sigmoid(gate).  scale defaults to 1 / sqrt(D)."""
-    _need_rows("attn_paged: q", q, kv.dtype, kv.device)
+    row = _token_stride("attn_paged: q", q, kv)
     T, H, D = q.shape
-    if D != kv.D:
-        raise ValueError(f"attn_paged: q of {D} dims, a cache of {kv.D}")
-    _need_cuda(o, lse, workspace)
     if o is None:
-        o = torch.empty((T, H, D), dtype=kv.dtype, device=q.device)
+        o = torch.empty((T, H, D), dtype=kv.dtype, device=kv.device)
+    elif o.shape != q.shape or not (o.is_cuda and o.is_contiguous()):
+        raise ValueError("attn_paged: o [tokens, H, D], contiguous")
     if lse is None:
-        lse = torch.empty((T, H), dtype=torch.float32, device=q.device)
-    if o.shape != q.shape or lse.numel() != T * H or lse.dtype != torch.float32:
-        raise ValueError("attn_paged: o [tokens, H, D], lse f32 [tokens, H]")
-    gr = gh = 0
+        lse = torch.empty((T, H), dtype=torch.float32, device=kv.device)
+    elif lse.numel() != T * H or not _is(lse, torch.float32):
+        raise ValueError("attn_paged: lse f32 [tokens, H], contiguous")
+    pg = gr = gh = 0
     if gate is not None:
-        if gate.dtype != torch.float32 or gate.shape != q.shape or gate.device != q.device or gate.stride(2) != 1:
+        gs = gate.stride()
+        if gate.dtype is not torch.float32 or gate.shape != q.shape or gate.device != kv.device or gs[2] != 1:
             raise ValueError("attn_paged: gate f32 [tokens, H, D] with inner stride 1")
-        gr, gh = gate.stride(0), gate.stride(1)
+        pg, gr, gh = gate.data_ptr(), gs[0], gs[1]
     if workspace is None:
-        workspace = attn_paged_workspace(batch, T, H, kv.KVH, D, q.device)
-    _lib.check(_lib.load().w4a8_attn_paged(
-        _ptr(q), q.stride(0) if T > 1 else H * D, H, kv.KVH, D, 1.0 / math.sqrt(D) if scale is None else scale,
-        _ptr(gate), gr, gh, batch.pq, batch.pl, batch.pt, batch.B, batch.per, T, batch.max_q, batch.max_kv, kv.pk, kv.pv,
-        *kv.layout, _ptr(o), _TYPES.get(o.dtype, -1), _ptr(lse), _ptr(workspace), workspace.numel(), _stream()))
+        workspace = attn_paged_workspace(batch, T, H, kv.KVH, D, kv.device)
+    elif not _is(workspace, torch.uint8):
+        raise ValueError("attn_paged: workspace uint8")
+    st = _lib.load().w4a8_attn_paged(
+        q.data_ptr(), row, H, kv.KVH, D, kv.scale if scale is None else scale, pg, gr, gh, batch.pq, batch.pl, batch.pt,
+        batch.B, batch.per, T, batch.max_q, batch.max_kv, kv.pk, kv.pv, *kv.layout, o.data_ptr(), _TYPES.get(o.dtype, -1),
+        lse.data_ptr(), workspace.data_ptr(), workspace.numel(), _raw_stream(kv.device))
+    if st:
+        _lib.check(st)
     return o, lse
 
 
@@ -423,20 +460,20 @@ def attn_weights_workspace(batch, H, KVH, device):
 def attn_weights(q, lse, kv, batch, acc, scale=None, workspace=None):
     """acc f32 [B, KVH, slots] += the attention weight each slot received from the new
     tokens (w4a8.h), with attn_paged's q, lse and scale.  Returns acc."""
-    _need_rows("attn_weights: q", q, kv.dtype, kv.device)
+    row = _token_stride("attn_weights: q", q, kv)
     T, H, D = q.shape
-    _need_cuda(lse, acc, workspace)
-    if D != kv.D or lse.numel() != T * H or lse.dtype != torch.float32:
-        raise ValueError("attn_weights: q [tokens, H, D] of the cache's D, lse f32 [tokens, H]")
-    if acc.dtype != torch.float32 or acc.dim() != 3 or acc.shape[:2] != (batch.B, kv.KVH):
-        raise ValueError("attn_weights: acc f32 [B, KVH, slots]")
+    if lse.numel() != T * H or not (_is(lse, torch.float32) or not T):
+        raise ValueError("attn_weights: lse f32 [tokens, H], contiguous")
+    if acc.dim() != 3 or acc.shape[0] != batch.B or acc.shape[1] != kv.KVH or not _is(acc, torch.float32):
+        raise ValueError("attn_weights: acc f32 [B, KVH, slots], contiguous")
     if workspace is None:
-        workspace = attn_weights_workspace(batch, H, kv.KVH, q.device)
-    _lib.check(_lib.load().w4a8_attn_weights(
-        _ptr(q), q.stride(0) if T > 1 else H * D, _ptr(lse), H, kv.KVH, D,
-        1.0 / math.sqrt(D) if scale is None else scale, batch.pq, batch.pl, batch.pt, batch.B, batch.per, T,
-        batch.max_q, batch.max_kv, kv.pk, *kv.layout, _ptr(acc), acc.shape[2], _ptr(workspace),
-        0 if workspace is None else workspace.numel(), _stream()))
+        workspace = attn_weights_workspace(batch, H, kv.KVH, kv.device)
+    st = _lib.load().w4a8_attn_weights(
+        q.data_ptr(), row, lse.data_ptr(), H, kv.KVH, D, kv.scale if scale is None else scale, batch.pq, batch.pl, batch.pt,
+        batch.B, batch.per, T, batch.max_q, batch.max_kv, kv.pk, *kv.layout, acc.data_ptr(), acc.shape[2],
+        _opt(workspace, torch.uint8, "workspace"), 0 if workspace is None else workspace.numel(), _raw_stream(kv.device))
+    if st:
+        _lib.check(st)
     return acc
 
 
@@ -452,27 +489,36 @@ def kv_evict(kv, batch, acc, pos, keep, protect_from, sink=0, acc_out=None, pos_
     in place in the cache; acc f32 and pos int32 [B, KVH, slots].  Returns (acc_out, pos_out,
     len_out): acc_out and pos_out default to acc and pos themselves, len_out to a new tensor
     (it may not be batch.kv_len)."""
-    _need_cuda(acc, pos, keep, protect_from, acc_out, pos_out, len_out, workspace)
-    acc_out = acc if acc_out is None else acc_out
-    pos_out = pos if pos_out is None else pos_out
-    if len_out is None:
-        len_out = torch.empty_like(batch.kv_len)
-    if acc.dtype != torch.float32 or acc.dim() != 3 or acc.shape[:2] != (batch.B, kv.KVH) or pos.shape != acc.shape:
-        raise ValueError("kv_evict: acc f32 and pos int32 [B, KVH, slots]")
-    if acc_out.shape != acc.shape or pos_out.shape != acc.shape or acc_out.dtype != torch.float32:
-        raise ValueError("kv_evict: acc_out and pos_out as acc and pos")
-    for t, n in ((pos, 0), (pos_out, 0), (keep, batch.B), (protect_from, batch.B), (len_out, batch.B)):
-        if t.dtype != torch.int32 or (n and t.numel() != n):
-            raise ValueError("kv_evict: pos int32 as acc; keep, protect_from and len_out int32 [B]")
-    slots = acc.shape[2]
+    shape = acc.shape
+    if len(shape) != 3 or shape[0] != batch.B or shape[1] != kv.KVH or not _is(acc, torch.float32) or \
+            pos.shape != shape or not _is(pos, torch.int32):
+        raise ValueError("kv_evict: acc f32 and pos int32 [B, KVH, slots], contiguous")
+    slots = shape[2]
     if slots < batch.max_kv:
         raise ValueError(f"kv_evict: {slots} weights a head for up to {batch.max_kv} slots")
+    if acc_out is None:
+        acc_out = acc
+    elif acc_out.shape != shape or not _is(acc_out, torch.float32):
+        raise ValueError("kv_evict: acc_out as acc")
+    if pos_out is None:
+        pos_out = pos
+    elif pos_out.shape != shape or not _is(pos_out, torch.int32):
+        raise ValueError("kv_evict: pos_out as pos")
+    if len_out is None:
+        len_out = torch.empty_like(batch.kv_len)
+    for t in (keep, protect_from, len_out):
+        if t.numel() != batch.B or not _is(t, torch.int32):
+            raise ValueError("kv_evict: keep, protect_from and len_out int32 [B]")
     if workspace is None:
-        workspace = kv_evict_workspace(batch, kv.KVH, acc.device, slots)
-    _lib.check(_lib.load().w4a8_kv_evict(
-        kv.pk, kv.pv, *kv.layout, kv.KVH, kv.D, batch.pl, batch.pt, batch.B, batch.per, _ptr(acc), _ptr(pos), slots,
-        _ptr(keep), _ptr(protect_from), sink, _ptr(acc_out), _ptr(pos_out), _ptr(len_out), _ptr(workspace),
-        workspace.numel(), _stream()))
+        workspace = kv_evict_workspace(batch, kv.KVH, kv.device, slots)
+    elif not _is(workspace, torch.uint8):
+        raise ValueError("kv_evict: workspace uint8")
+    st = _lib.load().w4a8_kv_evict(
+        kv.pk, kv.pv, *kv.layout, kv.KVH, kv.D, batch.pl, batch.pt, batch.B, batch.per, acc.data_ptr(), pos.data_ptr(),
+        slots, keep.data_ptr(), protect_from.data_ptr(), sink, acc_out.data_ptr(), pos_out.data_ptr(), len_out.data_ptr(),
+        workspace.data_ptr(), workspace.numel(), _raw_stream(kv.device))
+    if st:
+        _lib.check(st)
     return acc_out, pos_out, len_out
 
 

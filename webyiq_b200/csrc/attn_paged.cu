@@ -736,7 +736,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
     } else {
         // ---- softmax, one thread a row, and the output ----
         // NQ = 2: a warpgroup a row tile, 64 slots a unit.  NQ = 1: two warpgroups, 64 of a unit's 128 slots each.
-        constexpr int kOut = 32;                              // columns of O in registers at a time
+        constexpr int kOut = 16;                              // columns of O in registers at a time
         constexpr int kUnits = NQ == 2 ? 2 : 1;               // units of a kv step
         const int grp = NQ == 2 ? warp >> 2 : 0, half = NQ == 2 ? 0 : warp >> 2, quarter = warp & 3;
         const int r = quarter * 32 + lane;  // row of the tile
@@ -898,23 +898,33 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
             if (g.parts == 1) {
                 if (any_live) {
                     const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll 1
-                    for (int col = d0; col < d1; col += kOut) {
-                        // a chunk's gates are asked for at once: a load's latency a chunk, not a load
-                        float o[kOut];
-                        float4 gate[kOut / 4];
-                        if (p.gate && live)
+                    // a chunk's gates are asked for a chunk ahead
+                    float4 gate[2][kOut / 4];
+                    auto ask = [&](int col, float4* to) {
+                        if (!p.gate || !live || col >= d1) return;
 #pragma unroll
-                            for (int e = 0; e < kOut; e += 8)
-                                if (col + e < d1) load_gate8(p, t, h, col + e, gate + e / 4);
+                        for (int e = 0; e < kOut; e += 8)
+                            if (col + e < d1) load_gate8(p, t, h, col + e, to + e / 4);
+                    };
+                    auto give = [&](int col, const float4* from) {
+                        if (col >= d1) return;
+                        float o[kOut];
 #pragma unroll
                         for (int e = 0; e < kOut; e += 16) tmem1_ld16(o_tm + col + e, o + e);
                         tmem1_wait_ld();
                         if (live)
 #pragma unroll
                             for (int e = 0; e < kOut; e += 8)
-                                if (col + e < d1) put8<T>(p, t, h, col + e, o + e, inv, gate + e / 4);
+                                if (col + e < d1) put8<T>(p, t, h, col + e, o + e, inv, from + e / 4);
                         __syncwarp();
+                    };
+                    ask(d0, gate[0]);
+#pragma unroll 1
+                    for (int col = d0; col < d1; col += 2 * kOut) {
+                        ask(col + kOut, gate[1]);
+                        give(col, gate[0]);
+                        ask(col + 2 * kOut, gate[0]);
+                        give(col + kOut, gate[1]);
                     }
                     if (live && half == 0 && p.lse)
                         p.lse[static_cast<size_t>(t) * p.H + h] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
@@ -1054,14 +1064,14 @@ w4a8_status launch_tc(const CUtensorMap& q, const CUtensorMap& k, const CUtensor
     const w4a8_status r =
         launch_pdl(what, attn_tc_kernel<T, NCH, NQ>, dim3(grid), dim3(Pl::kThreads), Pl::kSmem, st, q, k, v, p);
     if (r != W4A8_OK || grid == 1) return r;
-    // by how many threads a row's 8 columns are shared: about as many as fill the GPU for two items
+    // by how many threads a row's 8 columns are shared: few rows have many parts
     const int work = p.rows_cap * (p.D / 8);
     auto merge = [&](auto kernel, int pg) {
         const int per = kMergeThreads / pg;
         return launch_pdl(what, kernel, dim3(grid * NQ, (work + per - 1) / per), dim3(kMergeThreads), 0, st, p);
     };
-    if (work <= 512) return merge(attn_merge_kernel<T, NQ, 16>, 16);
-    if (work <= 2048) return merge(attn_merge_kernel<T, NQ, 4>, 4);
+    if (p.rows_cap <= 16) return merge(attn_merge_kernel<T, NQ, 16>, 16);
+    if (p.rows_cap < 64) return merge(attn_merge_kernel<T, NQ, 4>, 4);
     return merge(attn_merge_kernel<T, NQ, 1>, 1);
 }
 

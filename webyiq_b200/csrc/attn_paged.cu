@@ -57,7 +57,10 @@ constexpr uint32_t kChunkBytes = kTile * 128;  // 128 rows x 64 elements
 constexpr int kSegs = 4;
 constexpr int kMaxStages = 12;
 constexpr uint32_t kMiscBytes = 3072;
-constexpr int kItemCost = 2;  // an item's start and end (query load, epilogue), in kv steps
+// An item's start and end (query load, epilogue), in kv steps; a gate's loads lengthen its end.  Measured on 4001
+// tokens of 8 / 2 heads of 256: 152, 127, 119, 120 and 122 us with 2, 3, 4, 6 and 8 and a gate, 102, 101, 103, 104
+// and 107 without one; 48 single tokens 157, 151, 150, 151, 153.
+constexpr int kItemCost = 3, kGatedItemCost = 5;
 constexpr int kHalf = kTile / 2;  // scores of a row that one thread takes
 constexpr float kLazy = 8.0f;  // log2 of how far the maximum may pass its reference
 
@@ -71,6 +74,7 @@ struct AttnParams {
     int o_type;
     float* lse;
     int max_q, max_kv;
+    int item_cost;   // kItemCost or kGatedItemCost
     int box_rows;    // slots of a TMA box
     int box_tokens;  // tokens of one
     CacheOrder order;
@@ -128,16 +132,16 @@ __device__ __forceinline__ int kv_steps(int vis_last, int len) {
 
 // Length on the work line of one kv head of this lane's sequence (n tokens, 0 for none); a warp's call.
 // A sequence of many row tiles is summed by the whole warp.
-__device__ __forceinline__ int seq_length(const SeqSpan& s, int n, int tpc, int lane) {
+__device__ __forceinline__ int seq_length(const SeqSpan& s, int n, int tpc, int cost, int lane) {
     int total = 0;
     const bool many = n > 4 * tpc;
     if (!many)
-        for (int i = 0; i < n; i += tpc) total += kv_steps(s.len - s.n + min(i + tpc, n) - 1, s.len) + kItemCost;
+        for (int i = 0; i < n; i += tpc) total += kv_steps(s.len - s.n + min(i + tpc, n) - 1, s.len) + cost;
     for (unsigned todo = __ballot_sync(kFull, many); todo; todo &= todo - 1) {
         const int src = __ffs(todo) - 1;
         const int n1 = __shfl_sync(kFull, n, src), len = __shfl_sync(kFull, s.len, src), sn = __shfl_sync(kFull, s.n, src);
         int sum = 0;
-        for (int i = lane * tpc; i < n1; i += 32 * tpc) sum += kv_steps(len - sn + min(i + tpc, n1) - 1, len) + kItemCost;
+        for (int i = lane * tpc; i < n1; i += 32 * tpc) sum += kv_steps(len - sn + min(i + tpc, n1) - 1, len) + cost;
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
         if (lane == src) total = sum;
@@ -349,7 +353,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
         auto steps_of = [&](int b0) {
             SeqSpan s{};
             if (b0 + lane < p.b.batch) s = seq_span(p.b, p.c, b0 + lane);
-            return static_cast<long long>(seq_length(s, min(s.n, p.max_q), tpc, lane)) * p.KVH;
+            return static_cast<long long>(seq_length(s, min(s.n, p.max_q), tpc, p.item_cost, lane)) * p.KVH;
         };
         long long total = 0;
         for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
@@ -408,13 +412,13 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
         if (at < end) {
             s = seq_span(p.b, p.c, seq);
             n = min(s.n, p.max_q);
-            const long long per = __shfl_sync(kFull, seq_length(s, lane == 0 ? n : 0, tpc, lane), 0);
+            const long long per = __shfl_sync(kFull, seq_length(s, lane == 0 ? n : 0, tpc, p.item_cost, lane), 0);
             kh = static_cast<int>((at - base) / per);
             item = base + kh * per;
             for (;; i += 32 * tpc) {  // 32 row tiles at a time
                 const int first = i + lane * tpc;
                 steps = first < n ? kv_steps(s.len - s.n + min(first + tpc, n) - 1, s.len) : 0;
-                const int mine = first < n ? steps + kItemCost : 0;
+                const int mine = first < n ? steps + p.item_cost : 0;
                 int upto = mine;
 #pragma unroll
                 for (int off = 1; off < 32; off <<= 1) {
@@ -442,7 +446,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
             g.vis = s.len - s.n + i;
             g.len = s.len;
             // the item's steps come behind its fixed cost
-            const long long start = item + kItemCost;
+            const long long start = item + p.item_cost;
             g.j0 = static_cast<int>(max(at - start, 0ll));
             g.j1 = static_cast<int>(min(static_cast<long long>(steps), end - start));
             g.first = cta_of(start);
@@ -451,7 +455,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                 shared_item = make_int4(g.tok, g.n, g.kh, g.parts);
             }
             if (g.j1 > g.j0 && !publish(g)) break;
-            item += steps + kItemCost;
+            item += steps + p.item_cost;
             at = item;
             i += tpc;
             if (i >= n) {
@@ -1045,7 +1049,7 @@ Layout layout_of(int H, int KVH, int D, int batch, int max_q, int max_kv, int sm
     x.rows_cap = std::min(x.tpt, std::max(max_q, 1)) * G;
     const long long tiles = (static_cast<long long>(std::max(max_q, 1)) + x.nq * x.tpt - 1) / (x.nq * x.tpt);
     const long long steps = std::max((static_cast<long long>(max_kv) + kTile - 1) / kTile, 1ll);
-    const long long work = std::min(tiles * (steps + kItemCost), 1ll << 20) * KVH * batch;  // the longest the line can be
+    const long long work = std::min(tiles * (steps + kGatedItemCost), 1ll << 20) * KVH * batch;  // the longest the line can be
     x.grid = static_cast<int>(std::min<long long>(sms, work));
     x.items = (static_cast<size_t>(x.grid) * 16 + 255) / 256 * 256;
     x.slots = static_cast<size_t>(x.grid) * 2 * x.nq * x.rows_cap;
@@ -1152,6 +1156,7 @@ W4A8_API w4a8_status w4a8_attn_paged(const void* q, int32_t q_row_stride, int32_
     p.lse = lse;
     p.max_q = max_q;
     p.max_kv = max_kv;
+    p.item_cost = gate ? kGatedItemCost : kItemCost;
     p.box_rows = cache_box_rows(page);
     p.box_tokens = std::min(x.tpt, max_q);
     p.rows_cap = x.rows_cap;

@@ -349,28 +349,30 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
 
     if (warp == kLineWarp) {
         // ---- the work line: this CTA's stretch of it, segment by segment ----
-        // kv steps of sequence b0 + lane, all its kv heads
-        auto steps_of = [&](int b0) {
-            SeqSpan s{};
-            if (b0 + lane < p.b.batch) s = seq_span(p.b, p.c, b0 + lane);
-            return static_cast<long long>(seq_length(s, min(s.n, p.max_q), tpc, p.item_cost, lane)) * p.KVH;
+        // span and length, all its kv heads, of sequence b0 + lane
+        auto steps_of = [&](int b0, SeqSpan& o) {
+            o = SeqSpan{};
+            if (b0 + lane < p.b.batch) o = seq_span(p.b, p.c, b0 + lane);
+            return static_cast<long long>(seq_length(o, min(o.n, p.max_q), tpc, p.item_cost, lane)) * p.KVH;
         };
-        long long total = 0;
+        SeqSpan mine_span;
+        long long mine = 0, total = 0;
         for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
-            long long mine = steps_of(b0);
+            mine = steps_of(b0, mine_span);
+            long long sum = mine;
 #pragma unroll
-            for (int off = 16; off > 0; off >>= 1) mine += __shfl_xor_sync(kFull, mine, off);
-            total += mine;
+            for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
+            total += sum;
         }
         const long long ctas = min(static_cast<long long>(gridDim.x), total);
         const long long c = blockIdx.x;
         long long at = 0, end = 0;
         if (c < ctas) {
-            at = c * total / ctas;
-            end = (c + 1) * total / ctas;
+            at = line_div(c * total, ctas);
+            end = line_div((c + 1) * total, ctas);
         }
         // the CTA whose stretch holds step x
-        auto cta_of = [&](long long x) { return static_cast<int>(((x + 1) * ctas - 1) / total); };
+        auto cta_of = [&](long long x) { return static_cast<int>(line_div((x + 1) * ctas - 1, total)); };
         uint32_t sk = 0;
         bool ok = true;
         auto publish = [&](const Segment& s) -> bool {
@@ -384,12 +386,13 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
             ++sk;
             return true;
         };
-        // the sequence that holds step `at`, and the line position of its start
+        // the sequence that holds step `at`, its span and length, and the line position of its start
+        SeqSpan s{};
         int seq = 0;
-        long long base = 0;
+        long long base = 0, length = 0;
         if (at < end) {
             for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
-                const long long mine = steps_of(b0);
+                if (p.b.batch > 32) mine = steps_of(b0, mine_span);  // (one round: as above)
                 long long upto = mine;
 #pragma unroll
                 for (int off = 1; off < 32; off <<= 1) {
@@ -401,19 +404,20 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                     const int f = __ffs(past) - 1;
                     seq = b0 + f;
                     base += __shfl_sync(kFull, upto - mine, f);
+                    length = __shfl_sync(kFull, mine, f);
+                    s = SeqSpan{__shfl_sync(kFull, mine_span.t0, f), __shfl_sync(kFull, mine_span.n, f),
+                                __shfl_sync(kFull, mine_span.len, f)};
                     break;
                 }
                 base += __shfl_sync(kFull, upto, 31);
             }
         }
-        SeqSpan s{};
         int n = 0, kh = 0, i = 0, steps = 0;  // item: kv head kh, tokens from i
         long long item = base;                // its position
         if (at < end) {
-            s = seq_span(p.b, p.c, seq);
             n = min(s.n, p.max_q);
-            const long long per = __shfl_sync(kFull, seq_length(s, lane == 0 ? n : 0, tpc, p.item_cost, lane), 0);
-            kh = static_cast<int>((at - base) / per);
+            const long long per = line_div(length, p.KVH);
+            kh = static_cast<int>(line_div(at - base, per));
             item = base + kh * per;
             for (;; i += 32 * tpc) {  // 32 row tiles at a time
                 const int first = i + lane * tpc;
@@ -937,20 +941,21 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                 // a shared item: this CTA's part (neighbouring rows' 16 bytes lie side by side)
                 const size_t sl = part_slot<NQ>(blockIdx.x, g.first, grp);
                 float4* dst = p.part + sl * (p.D / 4) * p.rows_cap + r;
+                if (live && half == 0) p.ml[sl * p.rows_cap + r] = make_float2(m, l);
+                dst += static_cast<size_t>(d0 / 4) * p.rows_cap;
 #pragma unroll 1
-                for (int col = d0; col < d1; col += kOut) {
-                    float o[kOut];
-#pragma unroll
-                    for (int e = 0; e < kOut; e += 16) tmem1_ld16(o_tm + col + e, o + e);
+                for (int col = d0; col < d1; col += 16) {
+                    float o[16];
+                    tmem1_ld16(o_tm + col, o);
                     tmem1_wait_ld();
                     if (live) {
 #pragma unroll
-                        for (int e = 0; e < kOut; e += 4)
-                            if (col + e < d1) dst[static_cast<size_t>((col + e) / 4) * p.rows_cap] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        for (int e = 0; e < 4; ++e)
+                            dst[e * p.rows_cap] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                     }
+                    dst += 4 * p.rows_cap;
                     __syncwarp();
                 }
-                if (live && half == 0) p.ml[sl * p.rows_cap + r] = make_float2(m, l);
             }
             tc1_fence_before();
         }

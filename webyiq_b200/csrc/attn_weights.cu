@@ -190,28 +190,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         SeqSpan s;
         int n, tiles;
         long long total = 0;
+        long long mine = 0;
         for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
             span(b0 + lane, s, n, tiles);
-            long long mine = static_cast<long long>(seq_len(s, n, tiles)) * p.KVH;
+            mine = static_cast<long long>(seq_len(s, n, tiles)) * p.KVH;
+            long long sum = mine;
 #pragma unroll
-            for (int off = 16; off > 0; off >>= 1) mine += __shfl_xor_sync(kFull, mine, off);
-            total += mine;
+            for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
+            total += sum;
         }
         const long long ctas = min(static_cast<long long>(gridDim.x), total), me = blockIdx.x;
         long long at = 0, end = 0;
         if (me < ctas) {
-            at = me * total / ctas;
-            end = (me + 1) * total / ctas;
+            at = line_div(me * total, ctas);
+            end = line_div((me + 1) * total, ctas);
         }
         // the CTA whose stretch holds place x
-        auto cta_of = [&](long long x) { return static_cast<int>(((x + 1) * ctas - 1) / total); };
+        auto cta_of = [&](long long x) { return static_cast<int>(line_div((x + 1) * ctas - 1, total)); };
         int seq = 0, kh = 0, j = 0;
         long long pos = 0;  // start of item (seq, kh, j)
         bool ok = true;
         if (at < end) {
             for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
-                span(b0 + lane, s, n, tiles);
-                const long long mine = static_cast<long long>(seq_len(s, n, tiles)) * p.KVH;
+                if (p.b.batch > 32) {  // (one round: as above)
+                    span(b0 + lane, s, n, tiles);
+                    mine = static_cast<long long>(seq_len(s, n, tiles)) * p.KVH;
+                }
                 long long upto = mine;
 #pragma unroll
                 for (int off = 1; off < 32; off <<= 1) {
@@ -223,14 +227,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int f = __ffs(past) - 1;
                     seq = b0 + f;
                     pos += __shfl_sync(kFull, upto - mine, f);
-                    const long long per = __shfl_sync(kFull, mine, f) / p.KVH;
-                    kh = static_cast<int>((at - pos) / per);
+                    const long long per = line_div(__shfl_sync(kFull, mine, f), p.KVH);
+                    kh = static_cast<int>(line_div(at - pos, per));
                     pos += kh * per;
+                    s = SeqSpan{__shfl_sync(kFull, s.t0, f), __shfl_sync(kFull, s.n, f), __shfl_sync(kFull, s.len, f)};
+                    n = __shfl_sync(kFull, n, f);
+                    tiles = __shfl_sync(kFull, tiles, f);
                     break;
                 }
                 pos += __shfl_sync(kFull, upto, 31);
             }
-            span(seq, s, n, tiles);
             // the item that holds place `at`
             for (int j0 = 0; j0 < tiles; j0 += 32) {
                 const int len = j0 + lane < tiles ? item_len(s, n, j0 + lane) : 0;

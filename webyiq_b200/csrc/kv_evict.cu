@@ -8,13 +8,16 @@
 // a slot's place does not matter, and nothing else has to move.  Sources lie at n or
 // past it and destinations below n, so the moves are independent of one another.
 //
-// One CTA a (sequence, kv head): its keys are read once into shared memory (up to 51200
-// slots, in the workspace past that), the n-th largest key is found from histograms of
-// 11, 11 and 10 bits, of which the later two count the few keys left.  Then each thread
-// walks a stretch of consecutive slots, and one block-wide prefix sum each for ties, for
-// dropped slots below n and for kept slots past it gives them their numbers.  (With the
-// keys read again from memory for each of four 8-bit digits and a scan for every 1024
-// slots, 32 heads of 30011 slots took 87 us and the whole eviction 111; it now takes 49.)
+// A cluster of 1 to 8 CTAs takes a (sequence, kv head), a stretch of the slots each: the keys
+// are read once into shared memory (51200 of them a CTA, in the workspace past that), the
+// n-th largest is found from histograms of 11, 11 and 10 bits that the CTAs add up over
+// distributed shared memory.  Then each thread walks consecutive slots of its CTA's
+// stretch, and block-wide prefix sums, offset by the counts of the CTAs before, number the
+// ties, the dropped slots below n and the kept slots past it.  (One CTA a head with the
+// keys read again for each of four 8-bit digits and a scan for every 1024 slots took 87 us
+// for 32 heads of 30011 slots, with 11-bit digits and one read 33 us; clusters of 4 take about 20 us, and the whole eviction to 4096 slots 39 us.)
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "launch.cuh"
@@ -26,7 +29,8 @@ namespace {
 
 constexpr int kSelThreads = 1024;
 constexpr int kMoveThreads = 256;
-constexpr int kSharedKeys = 51200;  // slots whose keys fit in shared memory
+constexpr int kSharedKeys = 49152;  // slots whose keys fit in a CTA's shared memory
+constexpr int kMaxCluster = 8;
 constexpr int kBins = 2048;
 
 struct EvictParams {
@@ -80,13 +84,17 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* red, uint32
 }
 
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictParams p) {
+    namespace cg = cooperative_groups;
     extern __shared__ uint32_t shared_keys[];
-    __shared__ uint32_t hist[kBins];
+    __shared__ uint32_t hist[2][kBins];  // by turns, so that a pass may clear one while a neighbour still reads the other
     __shared__ uint32_t red[32];
     __shared__ uint32_t pick[3];
+    __shared__ uint32_t counts[3];  // dropped slots below n, kept slots past it, ties
     pdl_launch_dependents();
     pdl_wait();
-    const int kh = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    const int kh = blockIdx.x / ctas, seq = blockIdx.y, tid = threadIdx.x;
     const uint32_t cap = min(static_cast<uint32_t>(p.b.table_stride) * static_cast<uint32_t>(p.c.page),
                              static_cast<uint32_t>(p.stride));
     const int len = static_cast<int>(min(ld_dep(p.b.kv_len + seq), cap));
@@ -97,73 +105,80 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
     const uint32_t* pos = p.pos + row * p.stride;
     float* acc_out = p.acc_out + row * p.stride;
     uint32_t* pos_out = p.pos_out + row * p.stride;
-    if (kh == 0 && tid == 0) p.len_out[seq] = static_cast<uint32_t>(n);
-    if (n == len) {  // nothing goes
-        if (tid == 0) p.count[row] = 0;
-        if (acc_out != acc)
-            for (int j = tid; j < len; j += kSelThreads) acc_out[j] = ld_dep(acc + j);
-        if (pos_out != pos)
-            for (int j = tid; j < len; j += kSelThreads) pos_out[j] = ld_dep(pos + j);
+    if (kh == 0 && rank == 0 && tid == 0) p.len_out[seq] = static_cast<uint32_t>(n);
+    // this CTA's slots
+    const int part = (len + ctas - 1) / ctas;
+    const int s0 = min(rank * part, len), mine = min(part, len - s0);
+    if (n == len || n == 0) {  // nothing goes, or everything: the whole cluster leaves here
+        if (rank == 0 && tid == 0) p.count[row] = 0;
+        if (n > 0 && (acc_out != acc || pos_out != pos))
+            for (int j = s0 + tid; j < s0 + mine; j += kSelThreads) {
+                acc_out[j] = ld_dep(acc + j);
+                pos_out[j] = ld_dep(pos + j);
+            }
         return;
     }
-    if (n == 0) {
-        if (tid == 0) p.count[row] = 0;
-        return;
-    }
-    uint32_t* keys = p.keys ? p.keys + row * p.stride : shared_keys;
+    uint32_t* keys = p.keys ? p.keys + row * p.stride + s0 : shared_keys;
 
     // the n-th largest key: `prefix` down to its known bits, of the slots that match it so far the first `left` stay
     uint32_t prefix = 0, left = static_cast<uint32_t>(n), match = static_cast<uint32_t>(len);
     int low = 32;  // bits below the known ones
     for (int pass = 0; pass < 3 && left < match; ++pass) {
         const int bits = pass == 2 ? 10 : 11, shift = low - bits;
-        for (int b = tid; b < kBins; b += kSelThreads) hist[b] = 0;
+        uint32_t* h = hist[pass & 1];
+        for (int b = tid; b < kBins; b += kSelThreads) h[b] = 0;
         __syncthreads();
         auto count = [&](uint32_t key, bool live) {
             const uint32_t bin = (key >> shift) & ((1u << bits) - 1);
             int same;
             __match_all_sync(kFull, live ? bin : ~0u, &same);
             if (same) {  // ties come in runs: one addition for the warp
-                if (live && (tid & 31) == 0) atomicAdd(&hist[bin], 32u);
+                if (live && (tid & 31) == 0) atomicAdd(&h[bin], 32u);
             } else if (live) {
-                atomicAdd(&hist[bin], 1u);
+                atomicAdd(&h[bin], 1u);
             }
         };
         constexpr int kAhead = 8;
-        for (int j0 = 0; j0 < len; j0 += kSelThreads * kAhead) {
+        for (int j0 = 0; j0 < mine; j0 += kSelThreads * kAhead) {
             if (pass == 0) {
                 float w[kAhead];
                 uint32_t at[kAhead];
 #pragma unroll
                 for (int x = 0; x < kAhead; ++x) {
                     const int j = j0 + x * kSelThreads + tid;
-                    w[x] = j < len ? ld_dep(acc + j) : 0.f;
-                    at[x] = j < len ? ld_dep(pos + j) : 0u;
+                    w[x] = j < mine ? ld_dep(acc + s0 + j) : 0.f;
+                    at[x] = j < mine ? ld_dep(pos + s0 + j) : 0u;
                 }
 #pragma unroll
                 for (int x = 0; x < kAhead; ++x) {
                     const int j = j0 + x * kSelThreads + tid;
-                    if (j0 + x * kSelThreads >= len) break;
+                    if (j0 + x * kSelThreads >= mine) break;
                     const uint32_t key = rank_key(w[x], at[x], p.sink, from);
-                    if (j < len) keys[j] = key;
-                    count(key, j < len);
+                    if (j < mine) keys[j] = key;
+                    count(key, j < mine);
                 }
             } else {
 #pragma unroll
                 for (int x = 0; x < kAhead; ++x) {
                     const int j = j0 + x * kSelThreads + tid;
-                    if (j0 + x * kSelThreads >= len) break;
-                    const uint32_t key = j < len ? keys[j] : 0u;
-                    const bool live = j < len && (key >> low) == (prefix >> low);
+                    if (j0 + x * kSelThreads >= mine) break;
+                    const uint32_t key = j < mine ? keys[j] : 0u;
+                    const bool live = j < mine && (key >> low) == (prefix >> low);
                     if (__any_sync(kFull, live)) count(key, live);
                 }
             }
         }
-        __syncthreads();
+        cluster.sync();
         // from the top bin down: the bin in which the n-th largest lies
         uint32_t total;
         const int top = (1 << bits) - 1 - 2 * tid;  // this thread's two bins: top, top - 1
-        const uint32_t c0 = top > 0 ? hist[top] : 0u, c1 = top > 0 ? hist[top - 1] : 0u;
+        uint32_t c0 = 0, c1 = 0;
+        if (top > 0)
+            for (int q = 0; q < ctas; ++q) {
+                const uint32_t* other = cluster.map_shared_rank(h, q);
+                c0 += other[top];
+                c1 += other[top - 1];
+            }
         const uint32_t above = block_scan(c0 + c1, red, total);
         if (above < left && above + c0 >= left) {
             pick[0] = static_cast<uint32_t>(top);
@@ -183,48 +198,66 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
     __syncthreads();
     // Kept: keys above the prefix's bits, and of those that match it the first `left` by slot.
 
-    // a stretch of consecutive slots a thread; an odd length keeps the threads on different banks
-    const int run = ((len + kSelThreads - 1) / kSelThreads) | 1;
-    const int b0 = min(tid * run, len), b1 = min(b0 + run, len);
-    const uint32_t bar = low < 32 ? prefix >> low : 0u;
-    auto known = [&](uint32_t key) { return low < 32 ? key >> low : 0u; };
-    uint32_t ties = 0;
+    // consecutive slots a thread; an odd number keeps the threads on different banks
+    const int run = ((mine + kSelThreads - 1) / kSelThreads) | 1;
+    const int b0 = min(tid * run, mine), b1 = min(b0 + run, mine);
+    const uint32_t bar = prefix >> low;
     const bool some = left < match;  // not all of the matching slots stay
-    uint32_t total;
+    // what the CTAs before have of counts[which], after this one's total is in its own
+    auto before = [&](int which, uint32_t total) {
+        if (tid == 0) counts[which] = total;
+        cluster.sync();
+        uint32_t sum = 0;
+        for (int q = 0; q < rank; ++q) sum += *cluster.map_shared_rank(&counts[which], q);
+        return sum;
+    };
+    uint32_t total, ties = 0;
     if (some) {
-        for (int j = b0; j < b1; ++j) ties += known(keys[j]) == bar;
+        for (int j = b0; j < b1; ++j) ties += (keys[j] >> low) == bar;
         ties = block_scan(ties, red, total);
+        ties += before(2, total);
     }
     uint32_t holes = 0, sources = 0;
     for (int j = b0; j < b1; ++j) {
-        const uint32_t k = known(keys[j]);
+        const uint32_t k = keys[j] >> low;
         bool kept = k > bar;
         if (k == bar) kept = !some || ties++ < left;
         keys[j] = kept;
-        holes += j < n && !kept;
-        sources += j >= n && kept;
+        holes += s0 + j < n && !kept;
+        sources += s0 + j >= n && kept;
     }
-    uint32_t hole_at = block_scan(holes, red, total), source_at = block_scan(sources, red, total);
+    uint32_t source_total;
+    uint32_t hole_at = block_scan(holes, red, total);
+    uint32_t source_at = block_scan(sources, red, source_total);
+    if (tid == 0) {
+        counts[0] = total;
+        counts[1] = source_total;
+    }
+    cluster.sync();
+    uint32_t all = 0;
+    for (int q = 0; q < ctas; ++q) {
+        const uint32_t* other = cluster.map_shared_rank(counts, q);
+        if (q < rank) {
+            hole_at += other[0];
+            source_at += other[1];
+        }
+        all += other[0];
+    }
     uint32_t* dst = p.moves + row * 2 * (p.stride / 2 + 1);
     uint32_t* src = dst + p.stride / 2 + 1;
     for (int j = b0; j < b1; ++j) {
         const bool kept = keys[j] != 0;
-        if (j < n && !kept) dst[hole_at++] = static_cast<uint32_t>(j);
-        if (j >= n && kept) src[source_at++] = static_cast<uint32_t>(j);
+        if (s0 + j < n && !kept) dst[hole_at++] = static_cast<uint32_t>(s0 + j);
+        if (s0 + j >= n && kept) src[source_at++] = static_cast<uint32_t>(s0 + j);
     }
-    if (tid == 0) p.count[row] = total;  // sources, of which there are as many as holes
+    if (rank == 0 && tid == 0) p.count[row] = all;
     if (acc_out != acc || pos_out != pos)
-        for (int j = tid; j < n; j += kSelThreads)
+        for (int j = tid; j < min(mine, n - s0); j += kSelThreads)
             if (keys[j]) {
-                acc_out[j] = ld_dep(acc + j);
-                pos_out[j] = ld_dep(pos + j);
+                acc_out[s0 + j] = ld_dep(acc + s0 + j);
+                pos_out[s0 + j] = ld_dep(pos + s0 + j);
             }
-    __syncthreads();
-    for (uint32_t i = tid; i < total; i += kSelThreads) {
-        const uint32_t d = dst[i], s = src[i];
-        acc_out[d] = ld_dep(acc + s);
-        pos_out[d] = ld_dep(pos + s);
-    }
+    cluster.sync();  // no CTA leaves while a neighbour reads its counts
 }
 
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p) {
@@ -242,11 +275,39 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
         const int d = static_cast<int>(e - static_cast<uint64_t>(i) * per) * 8;
         const size_t a = slot_offset(p.b, p.c, seq, kh, static_cast<int>(ld_dep(src + i))) + d;
         const size_t b = slot_offset(p.b, p.c, seq, kh, static_cast<int>(ld_dep(dst + i))) + d;
+        if (d == 0) {  // the move's first piece takes the weight and the position along
+            const size_t from = row * p.stride + ld_dep(src + i), to = row * p.stride + ld_dep(dst + i);
+            p.acc_out[to] = ld_dep(p.acc + from);
+            p.pos_out[to] = ld_dep(p.pos + from);
+        }
         const uint4 k = ld_dep(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.c.k) + a));
         const uint4 v = ld_dep(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.c.v) + a));
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.c.k) + b) = k;
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.c.v) + b) = v;
     }
+}
+
+// A launch of clusters of `ctas` along x, with programmatic dependent launch.
+template <typename Kernel, typename... Args>
+w4a8_status launch_cluster(const char* what, Kernel kernel, dim3 grid, dim3 block, size_t smem, int ctas,
+                           cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = g_use_pdl ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (e != cudaSuccess) return set_error(W4A8_ECUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
+    return W4A8_OK;
 }
 
 }  // namespace
@@ -306,12 +367,18 @@ W4A8_API w4a8_status w4a8_kv_evict(void* k, void* v, int32_t dtype, int32_t page
     p.count = static_cast<uint32_t*>(workspace);
     p.moves = p.count + ((rows * 4 + 255) / 256) * 64;
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
-    p.keys = stride > kSharedKeys ? p.moves + (rows * 2 * (static_cast<size_t>(stride) / 2 + 1) + 63) / 64 * 64 : nullptr;
+    // as many CTAs a head as leave each 2048 slots and find an SM each, up to 8
+    int ctas = 1;
+    while (ctas < kMaxCluster && rows * ctas * 2 <= static_cast<size_t>(sm_count()) && stride / (ctas * 2) >= 2048) ctas *= 2;
+    const int part = (stride + ctas - 1) / ctas;
+    p.keys = part > kSharedKeys ? p.moves + (rows * 2 * (static_cast<size_t>(stride) / 2 + 1) + 63) / 64 * 64 : nullptr;
     static FuncAttr attr;
     st = ensure_smem(evict_select_kernel, attr, static_cast<size_t>(kSharedKeys) * 4, -1, what);
     if (st != W4A8_OK) return st;
-    st = launch_pdl(what, evict_select_kernel, dim3(KVH, batch), dim3(kSelThreads),
-                    p.keys ? 0 : static_cast<size_t>(stride) * 4, cs, p);
+    const dim3 grid(KVH * ctas, batch);
+    const size_t smem = p.keys ? 0 : static_cast<size_t>(part) * 4;
+    st = ctas == 1 ? launch_pdl(what, evict_select_kernel, grid, dim3(kSelThreads), smem, cs, p)
+                   : launch_cluster(what, evict_select_kernel, grid, dim3(kSelThreads), smem, ctas, cs, p);
     if (st != W4A8_OK) return st;
     // enough CTAs to fill the GPU, no more a head than its most moves take
     const long long most = (static_cast<long long>(stride) / 2 + 1) * (D / 8);

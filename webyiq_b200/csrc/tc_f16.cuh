@@ -147,6 +147,13 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// a / b for places on a work line, which nearly always fit 32 bits (a 64-bit division is
+// some hundreds of clocks, and a kernel's start waits for several of them).
+__device__ __forceinline__ long long line_div(long long a, long long b) {
+    if (static_cast<unsigned long long>(a | b) >> 32) return a / b;
+    return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+}
+
 // Bounded waits of a kernel's roles: one that gives up sets the device error word and
 // the CTA's abort flag, and every role then leaves its loop.
 struct Bail {

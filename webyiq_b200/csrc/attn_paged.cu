@@ -353,26 +353,26 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
         auto steps_of = [&](int b0, SeqSpan& o) {
             o = SeqSpan{};
             if (b0 + lane < p.b.batch) o = seq_span(p.b, p.c, b0 + lane);
-            return static_cast<long long>(seq_length(o, min(o.n, p.max_q), tpc, p.item_cost, lane)) * p.KVH;
+            return seq_length(o, min(o.n, p.max_q), tpc, p.item_cost, lane) * p.KVH;
         };
         SeqSpan mine_span;
-        long long mine = 0, total = 0;
+        int mine = 0, total = 0;
         for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
             mine = steps_of(b0, mine_span);
-            long long sum = mine;
+            int sum = mine;
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
             total += sum;
         }
-        const long long ctas = min(static_cast<long long>(gridDim.x), total);
-        const long long c = blockIdx.x;
-        long long at = 0, end = 0;
+        const int ctas = min(static_cast<int>(gridDim.x), total);
+        const int c = blockIdx.x;
+        int at = 0, end = 0;
         if (c < ctas) {
-            at = line_div(c * total, ctas);
-            end = line_div((c + 1) * total, ctas);
+            at = line_mul_div(c, total, ctas);
+            end = line_mul_div(c + 1, total, ctas);
         }
         // the CTA whose stretch holds step x
-        auto cta_of = [&](long long x) { return static_cast<int>(line_div((x + 1) * ctas - 1, total)); };
+        auto cta_of = [&](int x) { return line_mul_div(x + 1, ctas, total, 1); };
         uint32_t sk = 0;
         bool ok = true;
         auto publish = [&](const Segment& s) -> bool {
@@ -388,15 +388,14 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
         };
         // the sequence that holds step `at`, its span and length, and the line position of its start
         SeqSpan s{};
-        int seq = 0;
-        long long base = 0, length = 0;
+        int seq = 0, base = 0, length = 0;
         if (at < end) {
             for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
                 if (p.b.batch > 32) mine = steps_of(b0, mine_span);  // (one round: as above)
-                long long upto = mine;
+                int upto = mine;
 #pragma unroll
                 for (int off = 1; off < 32; off <<= 1) {
-                    const long long y = __shfl_up_sync(kFull, upto, off);
+                    const int y = __shfl_up_sync(kFull, upto, off);
                     if (lane >= off) upto += y;
                 }
                 const unsigned past = __ballot_sync(kFull, base + upto > at);
@@ -413,13 +412,14 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
             }
         }
         int n = 0, kh = 0, i = 0, steps = 0;  // item: kv head kh, tokens from i
-        long long item = base;                // its position
+        int item = base;                      // its position
         if (at < end) {
             n = min(s.n, p.max_q);
-            const long long per = line_div(length, p.KVH);
-            kh = static_cast<int>(line_div(at - base, per));
+            const int per = length / p.KVH;
+            kh = (at - base) / per;
             item = base + kh * per;
-            for (;; i += 32 * tpc) {  // 32 row tiles at a time
+            bool found = false;
+            for (; i < n; i += 32 * tpc) {  // 32 row tiles at a time
                 const int first = i + lane * tpc;
                 steps = first < n ? kv_steps(s.len - s.n + min(first + tpc, n) - 1, s.len) : 0;
                 const int mine = first < n ? steps + p.item_cost : 0;
@@ -435,10 +435,12 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                     i += f * tpc;
                     item += __shfl_sync(kFull, upto - mine, f);
                     steps = __shfl_sync(kFull, steps, f);
+                    found = true;
                     break;
                 }
                 item += __shfl_sync(kFull, upto, 31);
             }
+            if (!found) end = 0;  // (a line past 2^31)
         }
         int4 shared_item = make_int4(0, 0, 0, 0);
         while (item < end && ok) {
@@ -450,9 +452,9 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
             g.vis = s.len - s.n + i;
             g.len = s.len;
             // the item's steps come behind its fixed cost
-            const long long start = item + p.item_cost;
-            g.j0 = static_cast<int>(max(at - start, 0ll));
-            g.j1 = static_cast<int>(min(static_cast<long long>(steps), end - start));
+            const int start = item + p.item_cost;
+            g.j0 = max(at - start, 0);
+            g.j1 = min(steps, end - start);
             g.first = cta_of(start);
             g.parts = cta_of(start + steps - 1) - g.first + 1;
             if (g.parts > 1 && g.first == static_cast<int>(blockIdx.x)) {

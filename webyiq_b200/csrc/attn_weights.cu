@@ -189,37 +189,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         SeqSpan s;
         int n, tiles;
-        long long total = 0;
-        long long mine = 0;
+        int total = 0;
+        int mine = 0;
         for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
             span(b0 + lane, s, n, tiles);
-            mine = static_cast<long long>(seq_len(s, n, tiles)) * p.KVH;
-            long long sum = mine;
+            mine = (seq_len(s, n, tiles)) * p.KVH;
+            int sum = mine;
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
             total += sum;
         }
-        const long long ctas = min(static_cast<long long>(gridDim.x), total), me = blockIdx.x;
-        long long at = 0, end = 0;
+        const int ctas = min(static_cast<int>(gridDim.x), total), me = blockIdx.x;
+        int at = 0, end = 0;
         if (me < ctas) {
-            at = line_div(me * total, ctas);
-            end = line_div((me + 1) * total, ctas);
+            at = line_mul_div(me, total, ctas);
+            end = line_mul_div(me + 1, total, ctas);
         }
         // the CTA whose stretch holds place x
-        auto cta_of = [&](long long x) { return static_cast<int>(line_div((x + 1) * ctas - 1, total)); };
+        auto cta_of = [&](int x) { return line_mul_div(x + 1, ctas, total, 1); };
         int seq = 0, kh = 0, j = 0;
-        long long pos = 0;  // start of item (seq, kh, j)
+        int pos = 0;  // start of item (seq, kh, j)
         bool ok = true;
         if (at < end) {
             for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
                 if (p.b.batch > 32) {  // (one round: as above)
                     span(b0 + lane, s, n, tiles);
-                    mine = static_cast<long long>(seq_len(s, n, tiles)) * p.KVH;
+                    mine = (seq_len(s, n, tiles)) * p.KVH;
                 }
-                long long upto = mine;
+                int upto = mine;
 #pragma unroll
                 for (int off = 1; off < 32; off <<= 1) {
-                    const long long y = __shfl_up_sync(kFull, upto, off);
+                    const int y = __shfl_up_sync(kFull, upto, off);
                     if (lane >= off) upto += y;
                 }
                 const unsigned past = __ballot_sync(kFull, pos + upto > at);
@@ -227,8 +227,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int f = __ffs(past) - 1;
                     seq = b0 + f;
                     pos += __shfl_sync(kFull, upto - mine, f);
-                    const long long per = line_div(__shfl_sync(kFull, mine, f), p.KVH);
-                    kh = static_cast<int>(line_div(at - pos, per));
+                    const int per = __shfl_sync(kFull, mine, f) / p.KVH;
+                    kh = (at - pos) / per;
                     pos += kh * per;
                     s = SeqSpan{__shfl_sync(kFull, s.t0, f), __shfl_sync(kFull, s.n, f), __shfl_sync(kFull, s.len, f)};
                     n = __shfl_sync(kFull, n, f);
@@ -291,8 +291,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             it.len = min(s.len, p.acc_stride);
             it.j = j;
             const int i0 = first_row_tile(s, j, p.tpt), steps = max((n + p.tpt - 1) / p.tpt - i0, 0);
-            const long long start = pos + 1;
-            const int lo = static_cast<int>(max(at - start, 0ll)), hi = static_cast<int>(min(static_cast<long long>(steps), end - start));
+            const int start = pos + 1;
+            const int lo = max(at - start, 0), hi = min(steps, end - start);
             it.i0 = i0 + lo;
             it.steps = hi - lo;
             if (hi > lo) {

@@ -147,11 +147,12 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// a / b for places on a work line, which nearly always fit 32 bits (a 64-bit division is
-// some hundreds of clocks, and a kernel's start waits for several of them).
-__device__ __forceinline__ long long line_div(long long a, long long b) {
-    if (static_cast<unsigned long long>(a | b) >> 32) return a / b;
-    return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+// (a * b - less) / c for places on a work line, which are below 2^31 (that many kv steps
+// would take a day); the product nearly always fits 32 bits, and a 64-bit division is some
+// hundreds of clocks that a kernel's start would wait for.
+__device__ __forceinline__ int line_mul_div(int a, int b, int c, int less = 0) {
+    const unsigned long long x = static_cast<unsigned long long>(a) * static_cast<unsigned>(b) - less;
+    return static_cast<int>(x >> 32 ? x / static_cast<unsigned>(c) : static_cast<uint32_t>(x) / static_cast<uint32_t>(c));
 }
 
 // Bounded waits of a kernel's roles: one that gives up sets the device error word and

@@ -97,11 +97,16 @@ struct Segment {
     int first, parts;  // first CTA of the item, CTAs that share it
 };
 
-template <int NCH, int NQ>
+template <int NCH, int NQ, bool PAIR>
 struct Plan {
-    static constexpr int kCps = NCH == 4 ? 2 : NCH;  // 64-wide chunks of a ring stage
-    static constexpr int kParts = NCH / kCps;        // stages of a K or V tile
-    static constexpr uint32_t kStageBytes = kCps * kChunkBytes;
+    static constexpr int kCps = PAIR || NCH < 4 ? NCH : 2;  // 64-wide chunks of a ring stage
+    static constexpr int kParts = NCH / kCps;               // stages of a K or V tile
+    // a pair's CTA holds half of each tile: 64 slots of K, half the columns of V
+    static constexpr uint32_t kKChunk = PAIR ? kChunkBytes / 2 : kChunkBytes;
+    static constexpr int kVCps = PAIR ? NCH / 2 : kCps;
+    static constexpr uint32_t kStageBytes = kCps * kKChunk;
+    static constexpr int kTiles = PAIR ? 2 : NQ;  // row tiles of an item
+    static_assert(!PAIR || (NQ == 1 && NCH == 4), "pairs are for one row tile a CTA and the widest heads");
     static constexpr uint32_t kQBytes = NQ * NCH * kChunkBytes;
     static constexpr int kFit = static_cast<int>((227 * 1024 - kMiscBytes - kQBytes) / kStageBytes);
     static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
@@ -115,6 +120,7 @@ struct Bars {
     uint64_t full[kMaxStages], empty[kMaxStages];
     uint64_t s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][parity of the unit]
     uint64_t q_full, q_empty;
+    uint64_t peer_full[kMaxStages], peer_q;  // the pair's other CTA has its half (in CTA 0)
     uint64_t seg_full[kSegs], seg_empty[kSegs];
     uint64_t pair[4];     // [quarter]: the two warps that share its rows (NQ = 1)
     uint64_t turn[2][4];  // [row tile][quarter]: its exponentials' turn (NQ = 2)
@@ -285,11 +291,11 @@ __global__ void __launch_bounds__(kMergeThreads) attn_merge_kernel(const AttnPar
     if (col8 == 0 && p.lse) p.lse[static_cast<size_t>(t) * p.H + h] = sum == 0.f ? -INFINITY : top * p.scale + logf(sum);
 }
 
-template <typename T, int NCH, int NQ>
-__global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
+template <typename T, int NCH, int NQ, bool PAIR>
+__global__ void __launch_bounds__(Plan<NCH, NQ, PAIR>::kThreads, 1)
     attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                    const __grid_constant__ CUtensorMap tm_v, const AttnParams p) {
-    using P = Plan<NCH, NQ>;
+    using P = Plan<NCH, NQ, PAIR>;
     // the swizzled tiles want 1024-byte alignment, which dynamic shared memory has where there is no static
     extern __shared__ __align__(1024) unsigned char smem[];
     if (smem_u32(smem) & 1023) {
@@ -300,21 +306,26 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
     Bars& bars = *reinterpret_cast<Bars*>(ring + P::kStages * P::kStageBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int kTmaWarp = P::kSoftWarps, kMmaWarp = kTmaWarp + 1, kLineWarp = kTmaWarp + 3;
+    // who shares the work line: CTAs, or pairs of them
+    const int rank = PAIR ? static_cast<int>(pair_rank()) : 0;
+    const int me = PAIR ? blockIdx.x / 2 : blockIdx.x, everyone = PAIR ? gridDim.x / 2 : gridDim.x;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < P::kStages; ++s) {
+            mbar_init(&bars.peer_full[s], 1);
             mbar_init(&bars.full[s], 1);
             mbar_init(&bars.empty[s], 2);  // both MMA warps, whether they use the tile or not
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(&bars.s_full[0][i], 1);
-            mbar_init(&bars.p_full[0][i], NQ == 2 ? 4 : 8);
+            mbar_init(&bars.p_full[0][i], PAIR ? 16 : NQ == 2 ? 4 : 8);
             mbar_init(&bars.o_done[0][i], 1);
             mbar_init(&bars.pair[i], 2);
             mbar_init(&bars.turn[0][i], 1);
             mbar_init(&bars.turn[1][i], 1);
         }
         mbar_init(&bars.q_full, 1);
+        mbar_init(&bars.peer_q, 1);
         mbar_init(&bars.q_empty, 2);
         for (int i = 0; i < kSegs; ++i) {
             mbar_init(&bars.seg_full[i], 1);
@@ -323,8 +334,14 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
         bars.abort = 0;
         mbar_init_fence();
     }
-    if (warp == kMmaWarp) tmem1_alloc(&bars.tmem, 512);
+    if (warp == kMmaWarp) {
+        if (PAIR)
+            tmem2_alloc(&bars.tmem, 512);
+        else
+            tmem1_alloc(&bars.tmem, 512);
+    }
     tc1_fence_before();
+    if (PAIR) pair_sync();  // both CTAs' barriers are there
     __syncthreads();
     tc1_fence_after();
     const uint32_t tmem = bars.tmem;
@@ -333,7 +350,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
     pdl_wait();
 
     const Bail bail{&bars.abort, p.err};
-    const int tpc = NQ * p.tpt;  // tokens of an item
+    const int tpc = P::kTiles * p.tpt;  // tokens of an item
     // The next segment, for every role but the line's; false at the end.
     uint32_t sq = 0;
     auto next_seg = [&](Segment& s) -> bool {
@@ -364,8 +381,8 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
             for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
             total += sum;
         }
-        const int ctas = min(static_cast<int>(gridDim.x), total);
-        const int c = blockIdx.x;
+        const int ctas = min(everyone, total);
+        const int c = me;
         int at = 0, end = 0;
         if (c < ctas) {
             at = line_mul_div(c, total, ctas);
@@ -457,7 +474,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
             g.j1 = min(steps, end - start);
             g.first = cta_of(start);
             g.parts = cta_of(start + steps - 1) - g.first + 1;
-            if (g.parts > 1 && g.first == static_cast<int>(blockIdx.x)) {
+            if (g.parts > 1 && g.first == me) {
                 shared_item = make_int4(g.tok, g.n, g.kh, g.parts);
             }
             if (g.j1 > g.j0 && !publish(g)) break;
@@ -477,7 +494,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
             }
             if (item < end) steps = kv_steps(s.len - s.n + min(i + tpc, n) - 1, s.len);
         }
-        if (lane == 0) p.shared_items[blockIdx.x] = shared_item;
+        if (lane == 0 && rank == 0) p.shared_items[me] = shared_item;
         Segment stop{};
         if (ok) publish(stop);
     } else if (warp == kTmaWarp) {
@@ -489,7 +506,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
         uint32_t u = 0, qs = 0;  // kv steps so far, query loads so far
         const int boxes = kTile / p.box_rows;
         const uint32_t box_bytes = static_cast<uint32_t>(p.box_rows) * 128;
-        // page and row of this lane's box of step j
+        // page and row of this lane's box of step j; a pair's CTA takes the boxes of its 64 slots for K
         auto locate = [&](const Segment& g, int j, int& page, int& row, int& n) {
             const int s0 = j * kTile + lane * p.box_rows;
             n = min(boxes, max((g.len - j * kTile + p.box_rows - 1) / p.box_rows, 0));
@@ -501,23 +518,27 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                 row = s0 - pi * p.c.page;
             }
         };
-        auto load = [&](const CUtensorMap* map, uint32_t pos, int kh, int page, int row, int n) -> bool {
+        auto load = [&](const CUtensorMap* map, bool is_k, uint32_t pos, int kh, int page, int row, int n) -> bool {
+            const int first = PAIR && is_k ? rank * boxes / 2 : 0;  // this CTA's boxes: first .. first + count
+            const int count = max(PAIR && is_k ? min(n - first, boxes / 2) : n, 0);
+            const int cps = is_k ? P::kCps : P::kVCps;
+            const int x0 = PAIR && !is_k ? rank * P::kVCps * 64 : 0;
+            const uint32_t chunk = is_k ? P::kKChunk : kChunkBytes;
             for (int part = 0; part < P::kParts; ++part) {
                 const uint32_t st = (pos + part) % P::kStages;
                 ok = ok && !*bail.flag && bail.wait(&bars.empty[st], (((pos + part) / P::kStages) & 1) ^ 1);
                 if (!__all_sync(kFull, ok)) return ok = false;
                 if (lane == 0) {
-                    if (n > 0)
-                        mbar_expect_tx(&bars.full[st], static_cast<uint32_t>(n) * box_bytes * P::kCps);
+                    if (count > 0)
+                        mbar_expect_tx(&bars.full[st], static_cast<uint32_t>(count) * box_bytes * cps);
                     else
                         mbar_arrive(&bars.full[st]);
                 }
                 __syncwarp();
-                if (lane < n) {
-                    const uint32_t dst = smem_u32(ring + st * P::kStageBytes) + lane * box_bytes;
-#pragma unroll
-                    for (int ch = 0; ch < P::kCps; ++ch)
-                        tma_load_4d(dst + ch * kChunkBytes, map, (part * P::kCps + ch) * 64, p.order.pick(0, row, kh, page),
+                if (lane >= first && lane < first + count) {
+                    const uint32_t dst = smem_u32(ring + st * P::kStageBytes) + (lane - first) * box_bytes;
+                    for (int ch = 0; ch < cps; ++ch)
+                        tma_load_4d(dst + ch * chunk, map, x0 + (part * P::kCps + ch) * 64, p.order.pick(0, row, kh, page),
                                     p.order.pick(1, row, kh, page), p.order.pick(2, row, kh, page), &bars.full[st]);
                 }
                 pos_max = max(pos_max, pos + part + 1);
@@ -538,17 +559,17 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                 for (int t = 0; t < NQ; ++t)
                     for (int ch = 0; ch < NCH; ++ch)
                         tma_load_3d_at(smem_u32(smem + (t * NCH + ch) * kChunkBytes), &tm_q, ch * 64, g.kh * p.G,
-                                       g.tok + t * p.tpt, &bars.q_full);
+                                       g.tok + (t + rank) * p.tpt, &bars.q_full);
             }
             ++qs;
             for (int j = g.j0; j < g.j1 && ok; ++j, ++u) {
                 int page, row, n;
                 locate(g, j, page, row, n);
                 if (NQ == 2) {
-                    if (load(&tm_k, 2 * u * P::kParts, g.kh, page, row, n)) load(&tm_v, (2 * u + 1) * P::kParts, g.kh, page, row, n);
+                    if (load(&tm_k, true, 2 * u * P::kParts, g.kh, page, row, n)) load(&tm_v, false, (2 * u + 1) * P::kParts, g.kh, page, row, n);
                 } else {
-                    if (load(&tm_k, (u == 0 ? 0 : 2 * u - 1) * P::kParts, g.kh, page, row, n) && u > 0)
-                        load(&tm_v, 2 * u * P::kParts, vkh, vpage, vrow, vn);
+                    if (load(&tm_k, true, (u == 0 ? 0 : 2 * u - 1) * P::kParts, g.kh, page, row, n) && u > 0)
+                        load(&tm_v, false, 2 * u * P::kParts, vkh, vpage, vrow, vn);
                     vpage = page;
                     vrow = row;
                     vn = n;
@@ -556,7 +577,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                 }
             }
         }
-        if (NQ == 1 && ok && u > 0) load(&tm_v, 2 * u * P::kParts, vkh, vpage, vrow, vn);
+        if (NQ == 1 && ok && u > 0) load(&tm_v, false, 2 * u * P::kParts, vkh, vpage, vrow, vn);
         // no copy may still be landing when the CTA exits (a place that was skipped was filled one round earlier)
         for (uint32_t s = 0; s < P::kStages; ++s) {
             // the last fill of this stage
@@ -575,7 +596,8 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
     } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
         // ---- MMA: S(u) = Q K(u)^T once P of this buffer's previous unit has been used by O += P V ----
         const int w = warp - kMmaWarp;  // row tile (NQ = 2), or the parity of its units (NQ = 1)
-        constexpr uint32_t id_qk = idesc_f16<T>(NQ == 2 ? kHalf : kTile, false), id_pv = idesc_f16<T>(P::kCps * 64, true);
+        constexpr uint32_t id_qk = PAIR ? idesc_f16_pair<T>(kTile, false) : idesc_f16<T>(NQ == 2 ? kHalf : kTile, false);
+        constexpr uint32_t id_pv = PAIR ? idesc_f16_pair<T>(NCH * 64, true) : idesc_f16<T>(P::kCps * 64, true);
         const uint32_t s_tm = tmem + w * kTile;
         const uint32_t o_tm = tmem + kO + (NQ == 2 ? w * NCH * 64 : 0);
         const uint32_t q_sm = smem_u32(smem) + (NQ == 2 ? w * NCH * kChunkBytes : 0);
@@ -589,13 +611,18 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
         };
         auto tile_wait = [&](uint32_t pos) {
             for (int part = 0; part < P::kParts; ++part)
-                if (!wait(&bars.full[(pos + part) % P::kStages], ((pos + part) / P::kStages) & 1)) return false;
+                if (!wait(&bars.full[(pos + part) % P::kStages], ((pos + part) / P::kStages) & 1) ||
+                    (PAIR && rank == 0 && !wait(&bars.peer_full[(pos + part) % P::kStages], ((pos + part) / P::kStages) & 1)))
+                    return false;
             return true;
         };
         auto tile_skip = [&](uint32_t pos) {
             if (!tile_wait(pos)) return;
             if (lane == 0)
-                for (int part = 0; part < P::kParts; ++part) mbar_arrive(&bars.empty[(pos + part) % P::kStages]);
+                for (int part = 0; part < P::kParts; ++part) {
+                    mbar_arrive(&bars.empty[(pos + part) % P::kStages]);
+                    if (PAIR) mbar_arrive_at(&bars.empty[(pos + part) % P::kStages], 1);
+                }
             __syncwarp();
         };
         auto v_pos = [&](uint32_t u) { return (NQ == 2 ? 2 * u + 1 : 2 * u + 2) * P::kParts; };
@@ -607,7 +634,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                 unsigned char* v = ring + ((v_pos(u) + part) % P::kStages) * P::kStageBytes;
                 for (int e = valid * 8 + lane; e < kTile * 8; e += 32)
 #pragma unroll
-                    for (int ch = 0; ch < P::kCps; ++ch)
+                    for (int ch = 0; ch < P::kVCps; ++ch)
                         *reinterpret_cast<uint4*>(v + ch * kChunkBytes + e * 16) = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async();
@@ -624,7 +651,10 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                 const uint32_t v = smem_u32(ring + ((v_pos(u) + part) % P::kStages) * P::kStageBytes) + half * kHalf * 128;
 #pragma unroll
                 for (int kk = 0; kk < kSteps; ++kk)
-                    mma_f16_ts(o_tm + part * P::kCps * 64, p_tm + kk * 8, desc_mn_major(v + kk * 2048, kChunkBytes), id_pv,
+                    if (PAIR)
+                        mma_f16_ts_pair(o_tm, p_tm + kk * 8, desc_mn_major(v + kk * 2048, kChunkBytes), id_pv, !first || kk > 0);
+                    else
+                        mma_f16_ts(o_tm + part * P::kCps * 64, p_tm + kk * 8, desc_mn_major(v + kk * 2048, kChunkBytes), id_pv,
                                !first || kk > 0);
             }
         };
@@ -636,12 +666,22 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                 for (int ch = 0; ch < P::kCps; ++ch)
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        mma_f16_ss(s_tm + half * kHalf, desc_k_major(q_sm + (part * P::kCps + ch) * kChunkBytes + kk * 32),
+                        if (PAIR)
+                            mma_f16_ss_pair(s_tm, desc_k_major(q_sm + ch * kChunkBytes + kk * 32),
+                                            desc_k_major(k + ch * P::kKChunk + kk * 32), id_qk, ch + kk > 0);
+                        else
+                            mma_f16_ss(s_tm + half * kHalf, desc_k_major(q_sm + (part * P::kCps + ch) * kChunkBytes + kk * 32),
                                    desc_k_major(k + ch * kChunkBytes + kk * 32), id_qk, part + ch + kk > 0);
             }
         };
+        auto commit = [&](uint64_t* bar) {
+            if (PAIR)
+                tc2_commit_both(bar);
+            else
+                tc1_commit(bar);
+        };
         auto release = [&](uint32_t pos) {
-            for (int part = 0; part < P::kParts; ++part) tc1_commit(&bars.empty[(pos + part) % P::kStages]);
+            for (int part = 0; part < P::kParts; ++part) commit(&bars.empty[(pos + part) % P::kStages]);
         };
         uint32_t u = 0, segs = 0;
         Segment g;
@@ -692,7 +732,36 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                 if (pv(x) && lane == 0) pv_done(x);
                 __syncwarp();
             }
+        } else if (PAIR && rank == 1) {
+            // CTA 1 of a pair issues nothing: its first MMA warp passes each of its fills on to CTA 0, in the
+            // ring's order, the V rows past the sequence cleared
+            auto pass = [&](uint32_t pos) {
+                if (lane == 0) mbar_arrive_at(&bars.peer_full[pos % P::kStages], 0);
+                __syncwarp();
+            };
+            int valid = kTile;
+            auto v = [&](uint32_t x) {
+                if (!tile_wait(v_pos(x))) return;
+                clear(x, valid);
+                pass(v_pos(x));
+            };
+            while (ok && next_seg(g)) {
+                if (w == 1) continue;
+                if (!wait(&bars.q_full, segs & 1)) break;
+                if (lane == 0) mbar_arrive_at(&bars.peer_q, 0);
+                __syncwarp();
+                for (int j = g.j0; j < g.j1 && ok; ++j, ++u) {
+                    if (tile_wait(k_pos(u))) pass(k_pos(u));
+                    if (u > 0 && ok) v(u - 1);
+                    valid = max(min(g.len - j * kTile, kTile), 0);
+                }
+                ++segs;
+            }
+            if (ok && w == 0 && u > 0) v(u - 1);
         } else {
+            auto q_wait = [&](uint32_t s) {
+                return wait(&bars.q_full, s & 1) && (!PAIR || wait(&bars.peer_q, s & 1));
+            };
             // S(u) once P(u - 2) has been used; the units of one parity are this warp's
             auto own = [&](uint32_t x) { return (x & 1) == static_cast<uint32_t>(w); };
             auto pv = [&](uint32_t x, bool first, int valid) {
@@ -705,7 +774,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                 tc1_fence_after();
                 if (lane == 0) {
                     pv_mma(x, 0, first);
-                    tc1_commit(&bars.o_done[0][w]);
+                    commit(&bars.o_done[0][w]);
                     release(v_pos(x));
                 }
                 __syncwarp();
@@ -718,12 +787,12 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                     // in the ring's order: K(u) V(u - 1)
                     if (!own(u)) {
                         tile_skip(k_pos(u));
-                    } else if ((!fresh || wait(&bars.q_full, segs & 1)) && tile_wait(k_pos(u))) {
+                    } else if ((!fresh || q_wait(segs)) && tile_wait(k_pos(u))) {
                         fresh = false;
                         tc1_fence_after();
                         if (lane == 0) {
                             qk_mma(u, 0);
-                            tc1_commit(&bars.s_full[0][w]);
+                            commit(&bars.s_full[0][w]);
                             release(k_pos(u));
                         }
                         __syncwarp();
@@ -735,9 +804,9 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                 }
                 // through with the segment's Q: a warp that had no unit in it comes after its load all the
                 // same, or its arrival could count for the segment before
-                if (ok && fresh) wait(&bars.q_full, segs & 1);
+                if (ok && fresh) q_wait(segs);
                 if (!ok) break;
-                if (lane == 0) tc1_commit(&bars.q_empty);
+                if (lane == 0) commit(&bars.q_empty);
                 __syncwarp();
                 ++segs;
             }
@@ -749,6 +818,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
         constexpr int kOut = 16;                              // columns of O in registers at a time
         constexpr int kUnits = NQ == 2 ? 2 : 1;               // units of a kv step
         const int grp = NQ == 2 ? warp >> 2 : 0, half = NQ == 2 ? 0 : warp >> 2, quarter = warp & 3;
+        const int tile = PAIR ? rank : grp;  // row tile of the item
         const int r = quarter * 32 + lane;  // row of the tile
         const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t o_tm = tmem + lane_off + kO + grp * NCH * 64;
@@ -787,15 +857,15 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
         };
         Segment g;
         while (ok && next_seg(g)) {
-            const int toks = min(max(g.n - grp * p.tpt, 0), p.tpt);
+            const int toks = min(max(g.n - tile * p.tpt, 0), p.tpt);
             const bool live = tok_in < toks;  // (rows past tpt * G have tok_in >= tpt)
             const bool any_live = __any_sync(kFull, live);
-            const int lim = live ? g.vis + grp * p.tpt + tok_in : -1;  // last slot this row sees
+            const int lim = live ? g.vis + tile * p.tpt + tok_in : -1;  // last slot this row sees
             int least = live ? lim : 0x7fffffff;
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) least = min(least, __shfl_xor_sync(kFull, least, off));
             const int h = g.kh * p.G + head_in;
-            const int t = g.tok + grp * p.tpt + tok_in;
+            const int t = g.tok + tile * p.tpt + tok_in;
             if (p.gate && live && g.parts == 1) {
                 // the gate is wanted at the segment's end: towards L2 now
                 const char* at = reinterpret_cast<const char*>(p.gate + static_cast<size_t>(t) * p.gate_row +
@@ -896,7 +966,12 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                     tc1_fence_before();
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.p_full[grp][u & 1]);
+                if (lane == 0) {
+                    if (PAIR)
+                        mbar_arrive_at(&bars.p_full[0][u & 1], 0);
+                    else
+                        mbar_arrive(&bars.p_full[grp][u & 1]);
+                }
             }
             if (!ok) break;
             if (!o_wait(u - 1)) break;
@@ -941,7 +1016,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
                 }
             } else if (any_live) {
                 // a shared item: this CTA's part (neighbouring rows' 16 bytes lie side by side)
-                const size_t sl = part_slot<NQ>(blockIdx.x, g.first, grp);
+                const size_t sl = part_slot<P::kTiles>(me, g.first, tile);
                 float4* dst = p.part + sl * (p.D / 4) * p.rows_cap + r;
                 if (live && half == 0) p.ml[sl * p.rows_cap + r] = make_float2(m, l);
                 dst += static_cast<size_t>(d0 / 4) * p.rows_cap;
@@ -965,9 +1040,13 @@ __global__ void __launch_bounds__(Plan<NCH, NQ>::kThreads, 1)
 
     tc1_fence_before();
     __syncthreads();
+    if (PAIR) pair_sync();  // no CTA leaves while its peer may still signal it
     if (warp == kMmaWarp) {
         tc1_fence_after();
-        tmem1_dealloc(tmem, 512);
+        if (PAIR)
+            tmem2_dealloc(tmem, 512);
+        else
+            tmem1_dealloc(tmem, 512);
     }
 }
 
@@ -1003,13 +1082,13 @@ w4a8_status encode(CUtensorMap* map, int dtype, int rank, const void* base, cons
 }  // namespace
 
 w4a8_status encode_cache(CUtensorMap* map, CacheOrder* order, const void* base, const PagedCache& c, int KVH, int D,
-                         const char* what) {
+                         int box_rows, const char* what) {
     struct Dim {
         int id;
         cuuint64_t count, stride;
         cuuint32_t box;
     } d[3] = {{0, static_cast<cuuint64_t>(c.page), static_cast<cuuint64_t>(c.row_stride) * 2,
-               static_cast<cuuint32_t>(cache_box_rows(c.page))},
+               static_cast<cuuint32_t>(box_rows)},
               {1, static_cast<cuuint64_t>(KVH), static_cast<cuuint64_t>(c.head_stride) * 2, 1},
               {2, static_cast<cuuint64_t>(c.pages), static_cast<cuuint64_t>(c.page_stride) * 2, 1}};
     // a dimension of one has no stride of its own: it goes last
@@ -1040,9 +1119,40 @@ w4a8_status encode_queries(CUtensorMap* map, const void* q, int dtype, int H, in
 
 namespace {
 
+// Pairs of CTAs that the current device runs at once (its SMs in twos, less where a cluster of SMs has an odd
+// one), read once per device; half its SMs where that cannot be read.
+int pair_count(int sms) {
+    static std::atomic<int> counts[kMaxDevices];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return sms / 2;
+    int n = counts[dev].load(std::memory_order_relaxed);
+    if (n) return n;
+    using Pl = Plan<4, 1, true>;
+    static FuncAttr attr;
+    if (ensure_smem(attn_tc_kernel<__half, 4, 1, true>, attr, Pl::kSmem, -1, "w4a8_attn_paged") != W4A8_OK) return sms / 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (sms / 2));
+    cfg.blockDim = dim3(Pl::kThreads);
+    cfg.dynamicSmemBytes = Pl::kSmem;
+    cudaLaunchAttribute a[1];
+    a[0].id = cudaLaunchAttributeClusterDimension;
+    a[0].val.clusterDim.x = 2;
+    a[0].val.clusterDim.y = 1;
+    a[0].val.clusterDim.z = 1;
+    cfg.attrs = a;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, attn_tc_kernel<__half, 4, 1, true>, &cfg) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        n = sms / 2;
+    }
+    counts[dev].store(n, std::memory_order_relaxed);
+    return n;
+}
+
 // How a call is laid out on the GPU, from its sizes alone.
 struct Layout {
-    int nch, nq, tpt, rows_cap, grid;
+    int nch, nq, tpt, rows_cap, grid;  // grid: CTAs, or pairs of them
+    bool pair;
     size_t items, slots, bytes;
 };
 
@@ -1051,44 +1161,51 @@ Layout layout_of(int H, int KVH, int D, int batch, int max_q, int max_kv, int sm
     const int G = H / KVH;
     x.nch = (D + 63) / 64;
     x.tpt = kTile / G;
-    // two row tiles for each K and V tile where there are rows for both and O fits beside them
-    x.nq = x.nch <= 2 && static_cast<long long>(max_q) * G > kTile ? 2 : 1;
+    // Two row tiles for each K and V tile where there are rows for both: in one CTA where O fits beside them, in
+    // two for the widest heads, whose single CTAs would read 128 KB from L2 for 2048 clocks of MMA.
+    const bool many = static_cast<long long>(max_q) * G > kTile;
+    x.nq = many && x.nch <= 2 ? 2 : 1;
+    x.pair = many && x.nch == 4;
+    const int tiles_of = x.pair ? 2 : x.nq;
     x.rows_cap = std::min(x.tpt, std::max(max_q, 1)) * G;
-    const long long tiles = (static_cast<long long>(std::max(max_q, 1)) + x.nq * x.tpt - 1) / (x.nq * x.tpt);
+    const long long tiles = (static_cast<long long>(std::max(max_q, 1)) + tiles_of * x.tpt - 1) / (tiles_of * x.tpt);
     const long long steps = std::max((static_cast<long long>(max_kv) + kTile - 1) / kTile, 1ll);
     const long long work = std::min(tiles * (steps + kGatedItemCost), 1ll << 20) * KVH * batch;  // the longest the line can be
-    x.grid = static_cast<int>(std::min<long long>(sms, work));
+    x.grid = static_cast<int>(std::min<long long>(x.pair ? pair_count(sms) : sms, work));
     x.items = (static_cast<size_t>(x.grid) * 16 + 255) / 256 * 256;
-    x.slots = static_cast<size_t>(x.grid) * 2 * x.nq * x.rows_cap;
+    x.slots = static_cast<size_t>(x.grid) * 2 * tiles_of * x.rows_cap;
     x.bytes = x.items + (x.slots * 8 + 255) / 256 * 256 + x.slots * D * 4;
     return x;
 }
 
-template <typename T, int NCH, int NQ>
+template <typename T, int NCH, int NQ, bool PAIR = false>
 w4a8_status launch_tc(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const AttnParams& p, int grid,
                       cudaStream_t st) {
-    using Pl = Plan<NCH, NQ>;
+    using Pl = Plan<NCH, NQ, PAIR>;
     const char* what = "w4a8_attn_paged";
     static FuncAttr attr;
-    const w4a8_status s = ensure_smem(attn_tc_kernel<T, NCH, NQ>, attr, Pl::kSmem, -1, what);
+    const w4a8_status s = ensure_smem(attn_tc_kernel<T, NCH, NQ, PAIR>, attr, Pl::kSmem, -1, what);
     if (s != W4A8_OK) return s;
-    const w4a8_status r =
-        launch_pdl(what, attn_tc_kernel<T, NCH, NQ>, dim3(grid), dim3(Pl::kThreads), Pl::kSmem, st, q, k, v, p);
+    const w4a8_status r = PAIR ? launch_cluster(what, attn_tc_kernel<T, NCH, NQ, PAIR>, dim3(2 * grid), dim3(Pl::kThreads),
+                                                Pl::kSmem, 2, st, q, k, v, p)
+                               : launch_pdl(what, attn_tc_kernel<T, NCH, NQ, PAIR>, dim3(grid), dim3(Pl::kThreads), Pl::kSmem,
+                                            st, q, k, v, p);
     if (r != W4A8_OK || grid == 1) return r;
     // by how many threads a row's 8 columns are shared: few rows have many parts
     const int work = p.rows_cap * (p.D / 8);
     auto merge = [&](auto kernel, int pg) {
         const int per = kMergeThreads / pg;
-        return launch_pdl(what, kernel, dim3(grid * NQ, (work + per - 1) / per), dim3(kMergeThreads), 0, st, p);
+        return launch_pdl(what, kernel, dim3(grid * Pl::kTiles, (work + per - 1) / per), dim3(kMergeThreads), 0, st, p);
     };
-    if (p.rows_cap <= 16) return merge(attn_merge_kernel<T, NQ, 16>, 16);
-    if (p.rows_cap < 64) return merge(attn_merge_kernel<T, NQ, 4>, 4);
-    return merge(attn_merge_kernel<T, NQ, 1>, 1);
+    if (p.rows_cap <= 16) return merge(attn_merge_kernel<T, Pl::kTiles, 16>, 16);
+    if (p.rows_cap < 64) return merge(attn_merge_kernel<T, Pl::kTiles, 4>, 4);
+    return merge(attn_merge_kernel<T, Pl::kTiles, 1>, 1);
 }
 
 template <typename T>
-w4a8_status dispatch(int nch, int nq, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+w4a8_status dispatch(int nch, int nq, bool pair, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                      const AttnParams& p, int grid, cudaStream_t st) {
+    if (pair) return launch_tc<T, 4, 1, true>(q, k, v, p, grid, st);
     if (nq == 2) return nch == 1 ? launch_tc<T, 1, 2>(q, k, v, p, grid, st) : launch_tc<T, 2, 2>(q, k, v, p, grid, st);
     switch (nch) {
         case 1: return launch_tc<T, 1, 1>(q, k, v, p, grid, st);
@@ -1164,7 +1281,7 @@ W4A8_API w4a8_status w4a8_attn_paged(const void* q, int32_t q_row_stride, int32_
     p.max_q = max_q;
     p.max_kv = max_kv;
     p.item_cost = gate ? kGatedItemCost : kItemCost;
-    p.box_rows = cache_box_rows(page);
+    p.box_rows = std::min(cache_box_rows(page), x.pair ? kTile / 2 : kTile);  // a pair's CTA takes 64 slots of K
     p.box_tokens = std::min(x.tpt, max_q);
     p.rows_cap = x.rows_cap;
     p.shared_items = static_cast<int4*>(workspace);
@@ -1173,12 +1290,12 @@ W4A8_API w4a8_status w4a8_attn_paged(const void* q, int32_t q_row_stride, int32_
     p.err = device_error_word();
     CUtensorMap mq, mk, mv;
     st = encode_queries(&mq, q, dtype, H, D, q_row_stride, tokens, p.G, p.box_tokens, what);
-    if (st == W4A8_OK) st = encode_cache(&mk, &p.order, k, p.c, KVH, D, what);
-    if (st == W4A8_OK) st = encode_cache(&mv, &p.order, v, p.c, KVH, D, what);
+    if (st == W4A8_OK) st = encode_cache(&mk, &p.order, k, p.c, KVH, D, p.box_rows, what);
+    if (st == W4A8_OK) st = encode_cache(&mv, &p.order, v, p.c, KVH, D, p.box_rows, what);
     if (st != W4A8_OK) return st;
     cudaStream_t cs = static_cast<cudaStream_t>(stream);
-    return dtype == W4A8_F16 ? dispatch<__half>(x.nch, x.nq, mq, mk, mv, p, x.grid, cs)
-                             : dispatch<__nv_bfloat16>(x.nch, x.nq, mq, mk, mv, p, x.grid, cs);
+    return dtype == W4A8_F16 ? dispatch<__half>(x.nch, x.nq, x.pair, mq, mk, mv, p, x.grid, cs)
+                             : dispatch<__nv_bfloat16>(x.nch, x.nq, x.pair, mq, mk, mv, p, x.grid, cs);
 }
 
 }  // extern "C"

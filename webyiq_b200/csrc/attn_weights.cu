@@ -597,7 +597,7 @@ W4A8_API w4a8_status w4a8_attn_weights(const void* q, int32_t q_row_stride, cons
     p.part = need ? reinterpret_cast<float*>(p.shared_items + sm_count()) : nullptr;
     CUtensorMap mq, mk;
     st = encode_queries(&mq, q, dtype, H, D, q_row_stride, tokens, p.G, p.box_tokens, what);
-    if (st == W4A8_OK) st = encode_cache(&mk, &p.order, k, p.c, KVH, D, what);
+    if (st == W4A8_OK) st = encode_cache(&mk, &p.order, k, p.c, KVH, D, p.box_rows, what);
     if (st != W4A8_OK) return st;
     // as many CTAs as the line can have places
     const long long tiles = (static_cast<long long>(max_kv) + kTile - 1) / kTile;

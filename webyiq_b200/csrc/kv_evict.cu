@@ -287,29 +287,6 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
     }
 }
 
-// A launch of clusters of `ctas` along x, with programmatic dependent launch.
-template <typename Kernel, typename... Args>
-w4a8_status launch_cluster(const char* what, Kernel kernel, dim3 grid, dim3 block, size_t smem, int ctas,
-                           cudaStream_t stream, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = g_use_pdl ? 1 : 0;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-    if (e != cudaSuccess) return set_error(W4A8_ECUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
-    return W4A8_OK;
-}
-
 }  // namespace
 
 int sm_count();  // capi.cu

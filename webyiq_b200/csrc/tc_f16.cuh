@@ -118,6 +118,55 @@ __device__ __forceinline__ void tc1_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                  : "memory");
 }
+// The same for a pair of CTAs (cta_group::2): M = 256, each CTA's 128 rows of A and D its own,
+// half of B's N in each CTA's shared memory.  One thread of CTA 0 issues.
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc_f16_pair(int n, bool b_mn_major) {
+    return (idesc_f16<T>(n, b_mn_major) & 0x00ffffffu) | (static_cast<uint32_t>(256 >> 4) << 24);
+}
+__device__ __forceinline__ void mma_f16_ss_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts_pair(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// Arrives on this barrier of both CTAs once the pair's MMAs so far complete (a completion signal, not a load).
+__device__ __forceinline__ void tc2_commit_both(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                     smem_u32(bar)),
+                 "h"(static_cast<unsigned short>(3))
+                 : "memory");
+}
+__device__ __forceinline__ void tmem2_alloc(uint32_t* slot, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem2_dealloc(uint32_t taddr, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+__device__ __forceinline__ uint32_t pair_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void pair_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Arrival on a barrier of CTA `rank` of the pair, after what this thread has seen and written.
+__device__ __forceinline__ void mbar_arrive_at(uint64_t* bar, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(bar)), "r"(rank));
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(r) : "memory");
+}
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -180,7 +229,7 @@ struct CacheOrder {
     }
 };
 w4a8_status encode_cache(CUtensorMap* map, CacheOrder* order, const void* base, const PagedCache& c, int KVH, int D,
-                         const char* what);
+                         int box_rows, const char* what);
 // Query rows of one kv head as (64 elements, G heads, tokens) boxes: row = token * G + head.
 w4a8_status encode_queries(CUtensorMap* map, const void* q, int dtype, int H, int D, int row_stride, int tokens, int G,
                            int box_tokens, const char* what);

@@ -14,22 +14,35 @@
 //    into tensor memory over S as 16-bit pairs, O += P V with P as the MMA's A operand.
 //    K tiles are K-major operands and V tiles MN-major ones straight from the page
 //    layout: nothing is transposed.
-//  - Two threads share a row (a tensor memory lane), 64 of a step's scores each: maximum
-//    and sum need no shuffles, only an exchange of the two maxima through shared
-//    memory. (One thread a row left a scheduler two warps, which the exponentials' issue
-//    held up: 530 us against XXX for 2048 tokens over 16384 slots, 32 / 8 heads of 128.)
-//    The exponentials are taken against a reference that follows the maximum only when
+//  - A thread takes 64 scores of one row (a tensor memory lane) at a time: maximum and sum
+//    need no shuffles.  The exponentials are taken against a reference that follows the maximum only when
 //    it has grown by more than 2^8, so O is rarely rescaled; P <= 2^8 keeps its relative
 //    precision, and f32 sums divide the reference out at the end.
 //  - P is rounded to the cache's type (the tensor core wants A and B alike): a relative
 //    error of 2^-11 (f16) or 2^-8 (bf16) a weight, of the size of the output's own
 //    rounding.  Its sum is taken before that rounding.
-//  - NQ = 2: two row tiles share each K and V tile, two softmax warpgroups each (head sizes
-//    up to 128).  NQ = 1: one row tile and two softmax warpgroups, two S buffers so
-//    that the next scores are computed meanwhile (256-wide heads, whose O takes
-//    half of tensor memory, and calls of up to 128 rows a kv head).
-//  - Two threads issue MMAs, each for its own S buffer (units of one parity): a thread
-//    that waits or commits holds up its own MMAs only.
+//  - NQ = 2: two row tiles share each K and V tile, a softmax warpgroup each (head sizes up to
+//    128).  A tile's S is two halves of 64 slots, so that one's scores are computed while
+//    the other's weights are made, and the two tiles' warps take turns at the
+//    exponentials.  NQ = 1: one row tile, two S buffers of 128 slots, and two softmax
+//    warpgroups that split a row's scores and exchange their maxima through shared memory
+//    (wider heads, whose O takes half of tensor memory, and calls of up to 128 rows a kv
+//    head).  PAIR: two such CTAs share each K and V tile, half of it in the shared memory of
+//    each (cta_group::2), for heads past 192 with more than one row tile.
+//  - Two threads issue MMAs, each for its own S buffers: a thread that waits or commits
+//    holds up its own MMAs only.
+//
+// What bounds it, measured: 2048 tokens over 16384 slots, 32 / 8 heads of 128: 484 us, 1064
+// TFLOP/s (0.64 of the measured bf16 rate); the tensor pipe's control is busy 75% of the
+// time, because an MMA of N = 64 costs as much as one of N = 128.  (Whole steps of 128:
+// 530 us, the scores and the exponentials in turn.  Two warpgroups a tile: 628.  A quarter or
+// half of the exponentials by polynomial on the FMA pipe: 529, 543; the special
+// function unit is 52% busy and not the limit.)  256-wide heads: 2048 tokens over 16384
+// slots, 8 / 2 heads, in 247 us, 1042 TFLOP/s; a 4001-token prompt takes 90 us as pairs and
+// 102 as single CTAs, whose L2 reads (128 KB a step of 2048 clocks) were the limit.
+// Single tokens: 48 sequences, 888 MB, at 5.5 to 6.0 TB/s (0.84 to 0.92 of the measured copy
+// rate); one token over 100003 slots 46.6 us, of which about 15 are the line, the first
+// loads and the merge.
 //
 // Work split.  The kv steps of all (sequence, kv head, row tile) items lie on one line,
 // and each CTA takes an equal stretch of it, found on the device from the batch's

@@ -329,10 +329,9 @@ W4A8_API w4a8_status w4a8_deltanet(const float* proj, const float* conv_w, float
  * taken from them (a start to tokens, a length to table_stride * page, a page to pages):
  * a wrong entry gives wrong values and no access out of range.  max_q and max_kv bound
  * the new tokens and slots of any sequence: new tokens past max_q are not computed,
- * max_kv goes by the launch's size.  Slots
- * past a sequence's length may hold anything, NaN too.  tokens = 0 is a no-op.  The row
- * tiles (128 query rows of a kv head) of a call times the 128-slot tiles each sees stay
- * below 2^31 in all. */
+ * max_kv only sizes the launch.  Slots past a sequence's length may hold anything, NaN
+ * too.  tokens = 0 is a no-op.  The row tiles (128 query rows of a kv head) of a call
+ * times the 128-slot tiles each sees stay below 2^31 in all. */
 enum { W4A8_F16 = 0, W4A8_BF16 = 1, W4A8_F32 = 2 };
 
 /* Norm of queries and keys per head, rotation, and append to the cache, in one pass over

@@ -32,17 +32,19 @@
 //  - Two threads issue MMAs, each for its own S buffers: a thread that waits or commits
 //    holds up its own MMAs only.
 //
-// What bounds it, measured: 2048 tokens over 16384 slots, 32 / 8 heads of 128: 484 us, 1064
-// TFLOP/s (0.64 of the measured bf16 rate); the tensor pipe's control is busy 75% of the
+// What bounds it, measured: 2048 tokens over 16384 slots, 32 / 8 heads of 128: 480 to 495 us
+// in short runs, 1040 to 1074 TFLOP/s (0.62 to 0.64 of the measured bf16 burst rate), 550
+// us over seconds at the 1000 W limit (1715 MHz); the tensor pipe's control is busy 75% of the
 // time, because an MMA of N = 64 costs as much as one of N = 128.  (Whole steps of 128:
 // 530 us, the scores and the exponentials in turn.  Two warpgroups a tile: 628.  A quarter or
 // half of the exponentials by polynomial on the FMA pipe: 529, 543; the special
 // function unit is 52% busy and not the limit.)  256-wide heads: 2048 tokens over 16384
-// slots, 8 / 2 heads, in 247 us, 1042 TFLOP/s; a 4001-token prompt takes 90 us as pairs and
-// 102 as single CTAs, whose L2 reads (128 KB a step of 2048 clocks) were the limit.
+// slots, 8 / 2 heads, in 247 us as pairs, 1044 TFLOP/s, and 276 as single CTAs, which read
+// 128 KB from L2 a step of 2048 clocks; a 4001-token prompt 90 against 100, gated 113
+// against 117 (the gate's loads at the items' ends are the same in both).
 // Single tokens: 48 sequences, 888 MB, at 5.5 to 6.0 TB/s (0.84 to 0.92 of the measured copy
-// rate); one token over 100003 slots 46.6 us, of which about 15 are the line, the first
-// loads and the merge.
+// rate); one token over 100003 slots 46.6 us, 15 above its
+// bytes' time: the line, the first loads and the merge.
 //
 // Work split.  The kv steps of all (sequence, kv head, row tile) items lie on one line,
 // and each CTA takes an equal stretch of it, found on the device from the batch's

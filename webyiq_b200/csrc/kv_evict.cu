@@ -15,7 +15,8 @@
 // stretch, and block-wide prefix sums, offset by the counts of the CTAs before, number the
 // ties, the dropped slots below n and the kept slots past it.  (One CTA a head with the
 // keys read again for each of four 8-bit digits and a scan for every 1024 slots took 87 us
-// for 32 heads of 30011 slots, with 11-bit digits and one read 33 us; clusters of 4 take about 20 us, and the whole eviction to 4096 slots 39 us.)
+// for 32 heads of 30011 slots, with 11-bit digits and one read 36 us; clusters of
+// 4 take 22 us, and the whole eviction to 4096 slots 39 to 41 us.)
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -32,16 +32,19 @@
 //  - Two threads issue MMAs, each for its own S buffers: a thread that waits or commits
 //    holds up its own MMAs only.
 //
-// What bounds it, measured: 2048 tokens over 16384 slots, 32 / 8 heads of 128: 480 to 495 us
-// in short runs, 1040 to 1074 TFLOP/s (0.62 to 0.64 of the measured bf16 burst rate), 550
-// us over seconds at the 1000 W limit (1715 MHz); the tensor pipe's control is busy 75% of the
-// time, because an MMA of N = 64 costs as much as one of N = 128.  (Whole steps of 128:
-// 530 us, the scores and the exponentials in turn.  Two warpgroups a tile: 628.  A quarter or
-// half of the exponentials by polynomial on the FMA pipe: 529, 543; the special
-// function unit is 52% busy and not the limit.)  256-wide heads: 2048 tokens over 16384
+// What bounds it, measured: 2048 tokens over 16384 slots, 32 / 8 heads of 128: 446 us in
+// short runs, 1157 TFLOP/s (0.69 of the measured bf16 burst rate), more at the 1000 W limit.
+// Not one unit but the hand-overs between them: a warp's 64 exponentials take 512 clocks at
+// the unit's rate (611 with their sums and rounding), its half step about 1900, and S is ready in 99
+// of 100 half steps; heads of 64, with two thirds of the MMAs, still take 412 us.  An MMA
+// warp's delay counts, too: its waits read the abort flag only where a barrier is not
+// complete.  (Whole steps of 128: 530 us, before these two steps, the scores and the
+// exponentials in turn.  Two warpgroups a tile: 628.  A quarter or half of the
+// exponentials by polynomial on the FMA pipe: 529, 543 where 504 stood.  The order of
+// multiplies, exponentials, sums and roundings: no change.)  256-wide heads: 2048 tokens over 16384
 // slots, 8 / 2 heads, in 247 us as pairs, 1044 TFLOP/s, and 276 as single CTAs, which read
 // 128 KB from L2 a step of 2048 clocks; a 4001-token prompt 90 against 100, gated 113
-// against 117 (the gate's loads at the items' ends are the same in both).
+// against 117; now 87 and 109.
 // Single tokens: 48 sequences, 888 MB, at 5.5 to 6.0 TB/s (0.84 to 0.92 of the measured copy
 // rate); one token over 100003 slots 46.6 us, 15 above its
 // bytes' time: the line, the first loads and the merge.
@@ -71,6 +74,10 @@ constexpr int kTile = 128;                  // rows of a query tile, and slots o
 constexpr uint32_t kChunkBytes = kTile * 128;  // 128 rows x 64 elements
 constexpr int kSegs = 4;
 constexpr int kMaxStages = 12;
+// After how many of a half step's 64 weights the other row tile's warp may begin its own: the hand-over takes about as
+// long as the rest.  2048 tokens over 16384 slots, 64-wide heads: 415, 413, 413, 419 and 414 us with 16, 32, 48, 56 and
+// 64; 455 where the arrival does not depend on the weights, which the assembler then puts before them.
+constexpr int kPass = 48;
 constexpr uint32_t kMiscBytes = 3072;
 // An item's start and end (query load, epilogue), in kv steps; a gate's loads lengthen its end.  Measured on 4001
 // tokens of 8 / 2 heads of 256: 152, 127, 119, 120 and 122 us with 2, 3, 4, 6 and 8 and a gate, 102, 101, 103, 104
@@ -145,6 +152,15 @@ struct Bars {
     int abort;
 };
 static_assert(sizeof(Bars) <= kMiscBytes, "barriers exceed their space");
+
+// An arrival that waits for a value: nothing else keeps one behind arithmetic that it does not use.
+__device__ __forceinline__ void arrive_after(uint64_t* bar, uint32_t value) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %1, 0xffffffff;\n @p mbarrier.arrive.shared::cta.b64 _, [%0];\n"
+        " @!p mbarrier.arrive.shared::cta.b64 _, [%0];\n}\n" ::"r"(smem_u32(bar)),
+        "r"(value)
+        : "memory");
+}
 
 __device__ __forceinline__ int kv_steps(int vis_last, int len) {
     const int end = min(max(vis_last + 1, 0), len);
@@ -621,7 +637,12 @@ __global__ void __launch_bounds__(Plan<NCH, NQ, PAIR>::kThreads, 1)
         // always comes after that stage's phase before (a parity wait that is a phase early
         // would return at once); a tile that is the other warp's is released unused.
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            ok = ok && !*bail.flag && bail.wait(bar, parity);
+            // the flag only where the barrier is not complete: 2048 tokens over 16384 slots 478 -> 446 us, 4001-token
+            // prompts of pairs 90.5 -> 87.5; a single row tile a CTA, which waits for HBM, has nothing from it (46.6, 47.7)
+            if (NQ == 2 || PAIR)
+                ok = ok && bail.ready(bar, parity);
+            else
+                ok = ok && !*bail.flag && bail.wait(bar, parity);
             return ok = __all_sync(kFull, ok);
         };
         auto tile_wait = [&](uint32_t pos) {
@@ -902,12 +923,12 @@ __global__ void __launch_bounds__(Plan<NCH, NQ, PAIR>::kThreads, 1)
                     ok = !*bail.flag && bail.wait(&bars.turn[grp][quarter], (grp == 0 ? u - 1 : u) & 1);
                     return ok = __all_sync(kFull, ok);
                 };
-                auto pass_turn = [&]() {
-                    if (NQ == 2 && lane == 0) mbar_arrive(&bars.turn[grp ^ 1][quarter]);
+                auto pass_turn = [&](uint32_t after) {
+                    if (NQ == 2 && lane == 0) arrive_after(&bars.turn[grp ^ 1][quarter], after);
                 };
                 if (!any_live) {
                     if (!take_turn()) break;
-                    pass_turn();
+                    pass_turn(0);
                 } else {
                     // scores and weights of this thread: 64 columns, and 32 at the start of the unit's place
                     const uint32_t unit = tmem + lane_off + (NQ == 2 ? grp * kTile + (u & 1) * kHalf : (u & 1) * kTile);
@@ -973,8 +994,8 @@ __global__ void __launch_bounds__(Plan<NCH, NQ, PAIR>::kThreads, 1)
                         l1 = __fadd2_rn(l1, b);
                         w[i / 2] = Elem<T>::pack(a.x, a.y);
                         w[i / 2 + 1] = Elem<T>::pack(b.x, b.y);
+                        if (i + 4 == kPass) pass_turn(w[i / 2 + 1]);
                     }
-                    pass_turn();
                     tmem1_st32(p_tm, w);
                     l += (l0.x + l0.y) + (l1.x + l1.y);
                     tmem1_wait_st();

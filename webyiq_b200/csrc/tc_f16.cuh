@@ -209,6 +209,11 @@ __device__ __forceinline__ int line_mul_div(int a, int b, int c, int less = 0) {
 struct Bail {
     volatile int* flag;
     unsigned int* err;
+    // A wait that looks at the flag only where the barrier is not complete yet: a barrier that
+    // mostly is costs one test.
+    __device__ __forceinline__ bool ready(uint64_t* bar, uint32_t parity) const {
+        return mbar_test(bar, parity) || (!*flag && wait(bar, parity));
+    }
     __device__ bool wait(uint64_t* bar, uint32_t parity) const {
         if (mbar_wait(bar, parity)) return true;
         *flag = 1;

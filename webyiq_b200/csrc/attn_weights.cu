@@ -17,9 +17,10 @@
 // workspace, and a small kernel adds those in the order of the stretches.  Single tokens
 // are bound by HBM (K is read once), chunks by the exponentials: 128 x 128 of them take
 // the SM's 16 a clock 1024 clocks, the MMA half of that at 128-wide heads.  Measured: 1500
-// tokens over 8200 slots, 32 / 8 heads of 128, in 138 us (664 TFLOP/s, the
+// tokens over 8200 slots, 32 / 8 heads of 128, in 134 us (682 TFLOP/s, the
 // exponentials alone take 151 K clocks, 77 us at 1965 MHz; 182 with one MMA warp, whose barrier tests and commits left gaps, 251
-// with two softmax warpgroups); 16 single tokens over 56 MB in 18 us.
+// with two softmax warpgroups); 16 single tokens over 56 MB in 17.6 us.
+// (136 and 17.9 with the abort flag read before every wait, not only where one has to wait.)
 //
 // Warp roles: four softmax warpgroups that take row tiles in turn, an S buffer each, so
 // that one's waits and loads run beside the others' exponentials (two left the unit idle
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t items = 0;
     auto next_item = [&](Item& it) -> bool {
         const uint32_t i = items % kItems;
-        const bool ok = !*bail.flag && bail.wait(&sm.item_full[i], (items / kItems) & 1);
+        const bool ok = bail.ready(&sm.item_full[i], (items / kItems) & 1);
         if (!__all_sync(kFull, ok)) return false;
         it = sm.item[i];
         __syncwarp();
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t sent = 0;
         auto publish = [&](const Item& it) {
             const uint32_t i = sent % kItems;
-            ok = ok && !*bail.flag && bail.wait(&sm.item_empty[i], ((sent / kItems) & 1) ^ 1);
+            ok = ok && bail.ready(&sm.item_empty[i], ((sent / kItems) & 1) ^ 1);
             if (!__all_sync(kFull, ok)) return ok = false;
             if (lane == 0) {
                 sm.item[i] = it;
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             more = next_item(next);
             if (more) locate(next, page_next, row_next, n_next);
             const uint32_t ks = kn % p.k_stages;
-            ok = !*bail.flag && bail.wait(&sm.k_empty[ks], ((kn / p.k_stages) & 1) ^ 1);
+            ok = bail.ready(&sm.k_empty[ks], ((kn / p.k_stages) & 1) ^ 1);
             if (!(ok = __all_sync(kFull, ok))) break;
             if (lane == 0) mbar_expect_tx(&sm.k_full[ks], static_cast<uint32_t>(n) * box_bytes * p.nch);
             __syncwarp();
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ++kn;
             for (int i = it.i0; i < it.i0 + it.steps; ++i, ++qn) {
                 const uint32_t qs = qn % p.q_stages;
-                ok = !*bail.flag && bail.wait(&sm.q_empty[qs], ((qn / p.q_stages) & 1) ^ 1);
+                ok = bail.ready(&sm.q_empty[qs], ((qn / p.q_stages) & 1) ^ 1);
                 if (!(ok = __all_sync(kFull, ok))) break;
                 if (lane == 0) mbar_expect_tx(&sm.q_full[qs], q_load * p.nch);
                 __syncwarp();
@@ -372,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t kn = 0, sn = 0;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            ok = ok && !*bail.flag && bail.wait(bar, parity);
+            ok = ok && bail.ready(bar, parity);
             return ok = __all_sync(kFull, ok);
         };
         Item it;
@@ -440,9 +441,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 off[gt] = pre * -1.44269504088896340736f;
                 pre = offset(it, i + kGroups);
                 mbar_arrive(&sm.group[grp]);
-                ok = !*bail.flag && bail.wait(&sm.group[grp], turn & 1);
+                ok = bail.ready(&sm.group[grp], turn & 1);
                 ++turn;
-                ok = ok && !*bail.flag && bail.wait(&sm.s_full[grp], ((sn + i) / kGroups) & 1);
+                ok = ok && bail.ready(&sm.s_full[grp], ((sn + i) / kGroups) & 1);
                 if (!(ok = __all_sync(kFull, ok))) break;
                 tc1_fence_after();
                 const uint32_t s_tm = tmem + lane_off + grp * kTile;
@@ -499,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // the other groups hand their shares of the item to the first
                 const uint32_t d = done & 1, phase = (done >> 1) & 1;
                 ++done;
-                ok = !*bail.flag && bail.wait(grp ? &sm.sum_empty[d] : &sm.sum_full[d], grp ? phase ^ 1 : phase);
+                ok = bail.ready(grp ? &sm.sum_empty[d] : &sm.sum_full[d], grp ? phase ^ 1 : phase);
                 if (!(ok = __all_sync(kFull, ok))) break;
                 if (grp)
                     sm.sum[d][grp - 1][gt] = total;

@@ -102,10 +102,11 @@ def main():
     prompts = [300, 40, 150]
     cache = Cache(layer, len(prompts), slots=a.budget + 300)
     left = list(prompts)
+    gen = torch.Generator(device="cuda").manual_seed(1)
     for s in range(a.steps):
         news = [min(n, 128) if n else 1 for n in left]  # prompts in chunks of 128, then a token at a time
         left = [max(n - 128, 0) for n in left]
-        out = step(layer, cache, torch.randn(sum(news), layer.hidden, device="cuda"), news, budget=a.budget)
+        out = step(layer, cache, torch.randn((sum(news), layer.hidden), generator=gen, device="cuda"), news, budget=a.budget)
         if s < 4 or s == a.steps - 1:
             print(f"step {s}: new tokens {news}, slots {cache.len}, |y| {out['y'].norm().item():.3f}")
     ops.device_error()

@@ -609,7 +609,14 @@ __global__ void __launch_bounds__(Plan<NCH, NQ, PAIR>::kThreads, 1)
             }
         }
         if (NQ == 1 && ok && u > 0) load(&tm_v, false, 2 * u * P::kParts, vkh, vpage, vrow, vn);
-        // no copy may still be landing when the CTA exits (a place that was skipped was filled one round earlier)
+        // No copy may still be landing when the CTA exits, and no commit's arrival may still be on its way (in a
+        // pair, from the other CTA): nothing else waits for the last release of a stage, of Q or of a unit's P V.
+        // After a wait that gave up somewhere there is no knowing which will come.  (A place that was skipped was
+        // filled one round earlier.)
+        auto drained = [&](uint64_t* bar, uint32_t phase) {
+            ok = ok && !*bail.flag && bail.wait(bar, phase & 1);
+            ok = __all_sync(kFull, ok);
+        };
         for (uint32_t s = 0; s < P::kStages; ++s) {
             // the last fill of this stage
             uint32_t last = 0;
@@ -621,9 +628,19 @@ __global__ void __launch_bounds__(Plan<NCH, NQ, PAIR>::kThreads, 1)
                     any = true;
                 }
             }
-            if (any) mbar_wait(&bars.full[s], (last / P::kStages) & 1);
+            if (any) {
+                mbar_wait(&bars.full[s], (last / P::kStages) & 1);
+                drained(&bars.empty[s], last / P::kStages);
+            }
         }
-        if (qs > 0) mbar_wait(&bars.q_full, (qs - 1) & 1);
+        if (qs > 0) {
+            mbar_wait(&bars.q_full, (qs - 1) & 1);
+            drained(&bars.q_empty, qs - 1);
+        }
+        for (uint32_t i = 0; i < 2 * NQ; ++i) {  // [row tile][parity of the unit]
+            const uint32_t units = NQ == 2 ? u : (u + 1 - (i & 1)) / 2;
+            if (units > 0) drained(&bars.o_done[i >> 1][i & 1], units - 1);
+        }
     } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
         // ---- MMA: S(u) = Q K(u)^T once P of this buffer's previous unit has been used by O += P V ----
         const int w = warp - kMmaWarp;  // row tile (NQ = 2), or the parity of its units (NQ = 1)
@@ -1076,7 +1093,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ, PAIR>::kThreads, 1)
 
     tc1_fence_before();
     __syncthreads();
-    if (PAIR) pair_sync();  // no CTA leaves while its peer may still signal it
+    if (PAIR) pair_sync();  // no CTA leaves while its peer's threads may still signal it (commits: the TMA warp's last waits)
     if (warp == kMmaWarp) {
         tc1_fence_after();
         if (PAIR)

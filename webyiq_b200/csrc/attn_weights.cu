@@ -360,11 +360,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                                    lane * 64, it.kh * p.G, it.t0 + i * p.tpt, &sm.q_full[qs]);
             }
         }
-        // no copy may still be landing when the CTA exits
-        for (uint32_t x = kn > p.k_stages ? kn - p.k_stages : 0; x < kn; ++x)
-            mbar_wait(&sm.k_full[x % p.k_stages], (x / p.k_stages) & 1);
-        for (uint32_t x = qn > p.q_stages ? qn - p.q_stages : 0; x < qn; ++x)
-            mbar_wait(&sm.q_full[x % p.q_stages], (x / p.q_stages) & 1);
+        // no copy may still be landing when the CTA exits, and no commit's arrival (the last releases of the stages,
+        // which nothing else waits for) still be on its way; after a wait that gave up there is no knowing which will come
+        auto drain = [&](uint64_t* full, uint64_t* empty, uint32_t n, uint32_t stages) {
+            for (uint32_t x = n > stages ? n - stages : 0; x < n; ++x) {
+                mbar_wait(&full[x % stages], (x / stages) & 1);
+                ok = ok && !*bail.flag && bail.wait(&empty[x % stages], (x / stages) & 1);
+                ok = __all_sync(kFull, ok);
+            }
+        };
+        drain(sm.k_full, sm.k_empty, kn, p.k_stages);
+        drain(sm.q_full, sm.q_empty, qn, p.q_stages);
     } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
         // ---- MMA: S^T = K Q^T, the even row tiles from one warp and the odd ones from the other (a barrier
         //      test or a commit holds up its own thread's MMAs only).  Both follow every fill in order. ----

@@ -331,7 +331,8 @@ W4A8_API w4a8_status w4a8_deltanet(const float* proj, const float* conv_w, float
  * the new tokens and slots of any sequence: new tokens past max_q are not computed,
  * max_kv only sizes the launch.  Slots past a sequence's length may hold anything, NaN
  * too.  tokens = 0 is a no-op.  The row tiles (128 query rows of a kv head) of a call
- * times the 128-slot tiles each sees stay below 2^31 in all. */
+ * times the 128-slot tiles each sees stay below 2^31 in all: past that a call computes
+ * nothing and records code 32 in the device error word. */
 enum { W4A8_F16 = 0, W4A8_BF16 = 1, W4A8_F32 = 2 };
 
 /* Norm of queries and keys per head, rotation, and append to the cache, in one pass over
@@ -445,6 +446,8 @@ W4A8_API void w4a8_set_gemm_kernel(int tensor_core);
  * a tensor-core step to finish) is bounded; a wait that gives up records a code here and the kernel returns
  * without touching its outputs.  This call synchronizes `stream`, returns
  * W4A8_ETIMEOUT and the code if any was recorded (and clears it), else W4A8_OK.
+ * Code 32 is no wait: a paged call whose batch, read on the device, asked for more
+ * than it can count.
  * code may be NULL. */
 W4A8_API w4a8_status w4a8_device_error(uint32_t* code, void* stream);
 

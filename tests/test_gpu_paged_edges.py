@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import paged as opg
-from webyiq_b200 import ops
+from webyiq_b200 import W4A8Error, ops
 
 from test_gpu_paged import Case
 
@@ -32,3 +32,30 @@ def test_back_to_back(cuda, H, KVH, D, lens, news):
         got.append((o2, lse2, ops.attn_weights(c.q, lse2, c.kv, c.batch, torch.zeros_like(acc))))
     assert ops.device_error() == 0
     assert all(torch.equal(a, o) and torch.equal(b, lse) and torch.equal(w, acc) for a, b, w in got)
+
+
+def test_line_too_long(cuda):
+    """Lengths and starts whose work passes 2^31 steps (the page table leads all of it to one page): nothing is
+    computed, the device error word says why, and the next call is as ever."""
+    T, L = 1 << 17, 1 << 30
+    k = torch.zeros((1, 16, 1024, 16), dtype=torch.float16, device=cuda)
+    kv = ops.PagedKV(k, k.clone())
+
+    def i32(*a):
+        return torch.tensor(a, dtype=torch.int32, device=cuda)
+
+    batch = ops.PagedBatch(i32(0, T), i32(L), torch.zeros((1, 1 << 20), dtype=torch.int32, device=cuda), T, 1000)
+    q = torch.zeros((T, 16, 16), dtype=torch.float16, device=cuda)
+    o, lse = torch.full_like(q, 7), torch.full((T, 16), 7.0, device=cuda)
+    ops.attn_paged(q, kv, batch, o=o, lse=lse)
+    with pytest.raises(W4A8Error, match="0x20"):
+        ops.device_error()
+    assert (o == 7).all() and (lse == 7).all()
+    acc = torch.zeros((1, 16, 1 << 24), device=cuda)
+    ops.attn_weights(q, lse, kv, batch, acc)
+    with pytest.raises(W4A8Error, match="0x20"):
+        ops.device_error()
+    assert not acc.any()
+    c = Case(cuda, [300], [40], 8, 2, 128)
+    c.check(*ops.attn_paged(c.q, c.kv, c.batch))
+    assert ops.device_error() == 0

@@ -163,24 +163,22 @@ __device__ __forceinline__ void arrive_after(uint64_t* bar, uint32_t value) {
 }
 
 __device__ __forceinline__ int kv_steps(int vis_last, int len) {
-    const int end = min(max(vis_last + 1, 0), len);
-    return max((end + kTile - 1) / kTile, 1);  // a tile that sees nothing still writes its zeros
+    return (max(min(vis_last + 1, len), 1) - 1) / kTile + 1;  // a tile that sees nothing still writes its zeros
 }
 
 // Length on the work line of one kv head of this lane's sequence (n tokens, 0 for none); a warp's call.
 // A sequence of many row tiles is summed by the whole warp.
-__device__ __forceinline__ int seq_length(const SeqSpan& s, int n, int tpc, int cost, int lane) {
-    int total = 0;
+__device__ __forceinline__ long long seq_length(const SeqSpan& s, int n, int tpc, int cost, int lane) {
+    long long total = 0;
     const bool many = n > 4 * tpc;
     if (!many)
         for (int i = 0; i < n; i += tpc) total += kv_steps(s.len - s.n + min(i + tpc, n) - 1, s.len) + cost;
     for (unsigned todo = __ballot_sync(kFull, many); todo; todo &= todo - 1) {
         const int src = __ffs(todo) - 1;
         const int n1 = __shfl_sync(kFull, n, src), len = __shfl_sync(kFull, s.len, src), sn = __shfl_sync(kFull, s.n, src);
-        int sum = 0;
+        long long sum = 0;
         for (int i = lane * tpc; i < n1; i += 32 * tpc) sum += kv_steps(len - sn + min(i + tpc, n1) - 1, len) + cost;
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
+        sum = line_sum(sum);
         if (lane == src) total = sum;
     }
     return total;
@@ -401,17 +399,17 @@ __global__ void __launch_bounds__(Plan<NCH, NQ, PAIR>::kThreads, 1)
         auto steps_of = [&](int b0, SeqSpan& o) {
             o = SeqSpan{};
             if (b0 + lane < p.b.batch) o = seq_span(p.b, p.c, b0 + lane);
-            return seq_length(o, min(o.n, p.max_q), tpc, p.item_cost, lane) * p.KVH;
+            return line_heads(seq_length(o, min(o.n, p.max_q), tpc, p.item_cost, lane), p.KVH);
         };
         SeqSpan mine_span;
-        int mine = 0, total = 0;
+        int mine = 0;
+        long long whole = 0;
         for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
-            mine = steps_of(b0, mine_span);
-            int sum = mine;
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
-            total += sum;
+            const long long steps = steps_of(b0, mine_span);
+            whole += line_sum(steps);
+            mine = static_cast<int>(steps);  // (used where the whole fits)
         }
+        const int total = line_length(whole, p.err);
         const int ctas = min(everyone, total);
         const int c = me;
         int at = 0, end = 0;
@@ -439,7 +437,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ, PAIR>::kThreads, 1)
         int seq = 0, base = 0, length = 0;
         if (at < end) {
             for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
-                if (p.b.batch > 32) mine = steps_of(b0, mine_span);  // (one round: as above)
+                if (p.b.batch > 32) mine = static_cast<int>(steps_of(b0, mine_span));  // (one round: as above)
                 int upto = mine;
 #pragma unroll
                 for (int off = 1; off < 32; off <<= 1) {
@@ -466,7 +464,6 @@ __global__ void __launch_bounds__(Plan<NCH, NQ, PAIR>::kThreads, 1)
             const int per = length / p.KVH;
             kh = (at - base) / per;
             item = base + kh * per;
-            bool found = false;
             for (; i < n; i += 32 * tpc) {  // 32 row tiles at a time
                 const int first = i + lane * tpc;
                 steps = first < n ? kv_steps(s.len - s.n + min(first + tpc, n) - 1, s.len) : 0;
@@ -483,12 +480,10 @@ __global__ void __launch_bounds__(Plan<NCH, NQ, PAIR>::kThreads, 1)
                     i += f * tpc;
                     item += __shfl_sync(kFull, upto - mine, f);
                     steps = __shfl_sync(kFull, steps, f);
-                    found = true;
                     break;
                 }
                 item += __shfl_sync(kFull, upto, 31);
             }
-            if (!found) end = 0;  // (a line past 2^31)
         }
         int4 shared_item = make_int4(0, 0, 0, 0);
         while (item < end && ok) {

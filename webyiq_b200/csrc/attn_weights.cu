@@ -167,15 +167,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto span = [&](int b, SeqSpan& s, int& n, int& tiles) {
             s = b < p.b.batch ? seq_span(p.b, p.c, b) : SeqSpan{};
             n = min(s.n, p.max_q);
-            tiles = n > 0 ? (min(s.len, p.acc_stride) + kTile - 1) / kTile : 0;
+            const int slots = n > 0 ? min(s.len, p.acc_stride) : 0;
+            tiles = slots / kTile + (slots % kTile != 0);
         };
         auto item_len = [&](const SeqSpan& s, int n, int j) {
             return max((n + p.tpt - 1) / p.tpt - first_row_tile(s, j, p.tpt), 0) + 1;
         };
-        // length of one kv head of this lane's sequence
+        // length of this lane's sequence, all its kv heads
         auto seq_len = [&](const SeqSpan& s, int n, int tiles) {
             const bool many = n > p.tpt || n < s.n;
-            int total = tiles * 2;  // one row tile, which sees something of every slot tile
+            long long total = tiles * 2ll;  // one row tile, which sees something of every slot tile
             for (unsigned todo = __ballot_sync(kFull, many); todo; todo &= todo - 1) {
                 const int src = __ffs(todo) - 1;
                 SeqSpan o;
@@ -183,26 +184,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                 o.n = __shfl_sync(kFull, s.n, src);
                 o.len = __shfl_sync(kFull, s.len, src);
                 const int on = __shfl_sync(kFull, n, src), ot = __shfl_sync(kFull, tiles, src);
-                int sum = 0;
+                long long sum = 0;
                 for (int j = lane; j < ot; j += 32) sum += item_len(o, on, j);
-#pragma unroll
-                for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
+                sum = line_sum(sum);
                 if (lane == src) total = sum;
             }
-            return total;
+            return line_heads(total, p.KVH);
         };
         SeqSpan s;
         int n, tiles;
-        int total = 0;
         int mine = 0;
+        long long whole = 0;
         for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
             span(b0 + lane, s, n, tiles);
-            mine = (seq_len(s, n, tiles)) * p.KVH;
-            int sum = mine;
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
-            total += sum;
+            const long long places = seq_len(s, n, tiles);
+            whole += line_sum(places);
+            mine = static_cast<int>(places);  // (used where the whole fits)
         }
+        const int total = line_length(whole, p.err);
         const int ctas = min(static_cast<int>(gridDim.x), total), me = blockIdx.x;
         int at = 0, end = 0;
         if (me < ctas) {
@@ -218,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int b0 = 0; b0 < p.b.batch; b0 += 32) {
                 if (p.b.batch > 32) {  // (one round: as above)
                     span(b0 + lane, s, n, tiles);
-                    mine = (seq_len(s, n, tiles)) * p.KVH;
+                    mine = static_cast<int>(seq_len(s, n, tiles));
                 }
                 int upto = mine;
 #pragma unroll

@@ -183,6 +183,8 @@ w4a8_status device_error(unsigned int* code, cudaStream_t st) {
         if (e != cudaSuccess) return set_error(W4A8_ECUDA, "w4a8_device_error: %s", cudaGetErrorString(e));
     }
     if (code) *code = v;
+    if (v == DEV_ERR_ATTN_LINE)
+        return set_error(W4A8_ETIMEOUT, "a batch's attention work passes 2^31 steps: nothing computed (code 0x%x)", v);
     return v ? set_error(W4A8_ETIMEOUT, "a bounded device-side wait gave up (code 0x%x)", v) : W4A8_OK;
 }
 

@@ -196,8 +196,26 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// (a * b - less) / c for places on a work line, which are below 2^31 (that many kv steps
-// would take a day); the product nearly always fits 32 bits, and a 64-bit division is some
+// Sum over a warp of lengths on a work line, none negative.  What 32 bits hold (nearly every batch) is one
+// reduction; longer ones are summed in 64 bits, cut at 2^40, so that no sum of them wraps.
+__device__ __forceinline__ long long line_sum(long long x) {
+    if (!__any_sync(kFull, (x >> 25) != 0)) return __reduce_add_sync(kFull, static_cast<unsigned>(x));
+    x = min(x, 1ll << 40);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(kFull, x, off);
+    return x;
+}
+// A sequence's line for all of its kv heads.
+__device__ __forceinline__ long long line_heads(long long one, int KVH) { return min(min(one, 1ll << 33) * KVH, 1ll << 40); }
+// Length of a whole line as the places on it are counted, in 31 bits: a longer one is not walked at all (its places
+// would wrap, and with them the heads and tokens found from them); the device error word says so.
+__device__ __forceinline__ int line_length(long long total, unsigned int* err) {
+    if (total <= 0x7fffffffll) return static_cast<int>(total);
+    if ((threadIdx.x & 31) == 0) atomicOr(err, DEV_ERR_ATTN_LINE);
+    return 0;
+}
+
+// (a * b - less) / c for places on a work line, which are below 2^31; the product nearly always fits 32 bits, and a 64-bit division is some
 // hundreds of clocks that a kernel's start would wait for.
 __device__ __forceinline__ int line_mul_div(int a, int b, int c, int less = 0) {
     const unsigned long long x = static_cast<unsigned long long>(a) * static_cast<unsigned>(b) - less;

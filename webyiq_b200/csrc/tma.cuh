@@ -15,6 +15,7 @@ enum : unsigned int {
     DEV_ERR_SELFTEST = 4u,      // w4a8_selftest_wait_timeout: its wait gave up (as it must)
     DEV_ERR_XCHG_TIMEOUT = 8u,  // peer key exchange: a rank's flag never arrived
     DEV_ERR_ATTN_TIMEOUT = 16u,  // paged attention or its weights: a pipeline wait gave up
+    DEV_ERR_ATTN_LINE = 32u,     // the same: the batch's work line passes 2^31, nothing computed
 };
 
 // --- TMA bulk copies and mbarriers (no cluster multicast anywhere) -----------

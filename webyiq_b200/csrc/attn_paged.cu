@@ -135,6 +135,7 @@ struct Plan {
     static constexpr size_t kSmem = kQBytes + kStages * kStageBytes + kMiscBytes;
     static constexpr int kSoftWarps = 8;
     static constexpr int kThreads = (kSoftWarps + 4) * 32;
+    static_assert(kStages + 2 * NQ < 32, "a lane each for the last waits");
     static_assert(kStages >= 2 * kParts + (kParts == 1 ? 1 : 0), "ring too short");
 };
 
@@ -606,36 +607,35 @@ __global__ void __launch_bounds__(Plan<NCH, NQ, PAIR>::kThreads, 1)
         if (NQ == 1 && ok && u > 0) load(&tm_v, false, 2 * u * P::kParts, vkh, vpage, vrow, vn);
         // No copy may still be landing when the CTA exits, and no commit's arrival may still be on its way (in a
         // pair, from the other CTA): nothing else waits for the last release of a stage, of Q or of a unit's P V.
-        // After a wait that gave up somewhere there is no knowing which will come.  (A place that was skipped was
-        // filled one round earlier.)
-        auto drained = [&](uint64_t* bar, uint32_t phase) {
-            ok = ok && !*bail.flag && bail.wait(bar, phase & 1);
-            ok = __all_sync(kFull, ok);
-        };
-        for (uint32_t s = 0; s < P::kStages; ++s) {
-            // the last fill of this stage
-            uint32_t last = 0;
-            bool any = false;
-            for (uint32_t q = pos_max > 2 * P::kStages ? pos_max - 2 * P::kStages : 0; q < pos_max; ++q) {
-                const bool skipped = NQ == 1 && u > 0 && q >= (2 * u - 1) * P::kParts && q < 2 * u * P::kParts;
-                if (q % P::kStages == s && !skipped) {
-                    last = q;
-                    any = true;
+        // A lane takes a stage, a unit's parity of a row tile, or Q: one after another the waits would add a
+        // microsecond to the CTA's end.
+        uint64_t *landed = nullptr, *released = nullptr;
+        uint32_t phase = 0;
+        if (lane < P::kStages) {
+            if (pos_max > static_cast<uint32_t>(lane)) {
+                // the last fill of this stage (a place that was skipped was filled one round earlier)
+                uint32_t last = pos_max - 1 - (pos_max - 1 - lane) % P::kStages;
+                if (NQ == 1 && u > 0 && last >= (2 * u - 1) * P::kParts && last < 2 * u * P::kParts) last -= P::kStages;
+                if (static_cast<int>(last) >= 0) {
+                    landed = &bars.full[lane];
+                    released = &bars.empty[lane];
+                    phase = last / P::kStages;
                 }
             }
-            if (any) {
-                mbar_wait(&bars.full[s], (last / P::kStages) & 1);
-                drained(&bars.empty[s], last / P::kStages);
-            }
-        }
-        if (qs > 0) {
-            mbar_wait(&bars.q_full, (qs - 1) & 1);
-            drained(&bars.q_empty, qs - 1);
-        }
-        for (uint32_t i = 0; i < 2 * NQ; ++i) {  // [row tile][parity of the unit]
+        } else if (lane < P::kStages + 2 * NQ) {
+            const int i = lane - P::kStages;  // [row tile][parity]
             const uint32_t units = NQ == 2 ? u : (u + 1 - (i & 1)) / 2;
-            if (units > 0) drained(&bars.o_done[i >> 1][i & 1], units - 1);
+            if (units > 0) released = &bars.o_done[i >> 1][i & 1];
+            phase = units - 1;
+        } else if (lane == P::kStages + 2 * NQ && qs > 0) {
+            landed = &bars.q_full;
+            released = &bars.q_empty;
+            phase = qs - 1;
         }
+        if (landed) mbar_wait(landed, phase & 1);
+        // (after a wait that gave up there is no knowing which arrivals will come)
+        if (released && ok && !*bail.flag) bail.wait(released, phase & 1);
+        __syncwarp();
     } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
         // ---- MMA: S(u) = Q K(u)^T once P of this buffer's previous unit has been used by O += P V ----
         const int w = warp - kMmaWarp;  // row tile (NQ = 2), or the parity of its units (NQ = 1)

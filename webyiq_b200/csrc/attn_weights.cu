@@ -360,16 +360,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         // no copy may still be landing when the CTA exits, and no commit's arrival (the last releases of the stages,
-        // which nothing else waits for) still be on its way; after a wait that gave up there is no knowing which will come
-        auto drain = [&](uint64_t* full, uint64_t* empty, uint32_t n, uint32_t stages) {
-            for (uint32_t x = n > stages ? n - stages : 0; x < n; ++x) {
-                mbar_wait(&full[x % stages], (x / stages) & 1);
-                ok = ok && !*bail.flag && bail.wait(&empty[x % stages], (x / stages) & 1);
-                ok = __all_sync(kFull, ok);
-            }
-        };
-        drain(sm.k_full, sm.k_empty, kn, p.k_stages);
-        drain(sm.q_full, sm.q_empty, qn, p.q_stages);
+        // which nothing else waits for) still be on its way: a lane takes a stage
+        const bool of_q = lane >= kMaxStages;
+        const uint32_t stage = of_q ? lane - kMaxStages : lane, stages = of_q ? p.q_stages : p.k_stages, fills = of_q ? qn : kn;
+        if (stage < stages && stage < fills) {
+            const uint32_t last = (fills - 1 - stage) / stages;  // its last fill's phase
+            mbar_wait(of_q ? &sm.q_full[stage] : &sm.k_full[stage], last & 1);
+            // (after a wait that gave up there is no knowing which arrivals will come)
+            if (ok && !*bail.flag) bail.wait(of_q ? &sm.q_empty[stage] : &sm.k_empty[stage], last & 1);
+        }
+        __syncwarp();
     } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
         // ---- MMA: S^T = K Q^T, the even row tiles from one warp and the odd ones from the other (a barrier
         //      test or a commit holds up its own thread's MMAs only).  Both follow every fill in order. ----

@@ -361,7 +361,7 @@ W4A8_API w4a8_status w4a8_qk_norm_rope_kv(const float* qkv, int32_t qkv_row_stri
  * cache's, or W4A8_F32); lse f32[tokens, H] (natural log of the sum of exp(scale q k^T))
  * or NULL.  A token that sees nothing gets o = 0 and lse = -inf.  Scores, sums and
  * accumulators are f32; the weights are rounded to the cache's type before they
- * meet v.  k and v must be finite in the slots below a sequence's length: a weight of
+ * meet v (f16: to 2^-11 of a weight, or to 2^-32 of the row's largest where that is more).  k and v must be finite in the slots below a sequence's length: a weight of
  * zero times an infinity is NaN.
  * workspace: w4a8_attn_paged_workspace_bytes(...) bytes (of the current device), 16-byte
  * aligned, any contents; calls that share one must not overlap on the GPU. */

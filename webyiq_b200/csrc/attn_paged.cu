@@ -16,11 +16,15 @@
 //    layout: nothing is transposed.
 //  - A thread takes 64 scores of one row (a tensor memory lane) at a time: maximum and sum
 //    need no shuffles.  The exponentials are taken against a reference that follows the maximum only when
-//    it has grown by more than 2^8, so O is rarely rescaled; P <= 2^8 keeps its relative
-//    precision, and f32 sums divide the reference out at the end.
+//    it has grown by more than 2^8, so O is rarely rescaled, and f32 sums divide the
+//    reference out at the end.
 //  - P is rounded to the cache's type (the tensor core wants A and B alike): a relative
 //    error of 2^-11 (f16) or 2^-8 (bf16) a weight, of the size of the output's own
-//    rounding.  Its sum is taken before that rounding.
+//    rounding.  Its sum is taken before that rounding.  f16 weights are made 2^7 times as
+//    large, so that they fill its range up to 2^15: below 2^-21 of the row's largest weight
+//    they are subnormal, with an error of up to 2^-32 of it, N 2^-32 for N slots.  (Without
+//    the factor 2^-25: a cache beside one slot that takes most of the weight lost its part of
+//    the output where its scores lie 17 below.)  bf16 has f32's exponents.
 //  - NQ = 2: two row tiles share each K and V tile, a softmax warpgroup each (head sizes up to
 //    128).  A tile's S is two halves of 64 slots, so that one's scores are computed while
 //    the other's weights are made, and the two tiles' warps take turns at the
@@ -85,6 +89,16 @@ constexpr uint32_t kMiscBytes = 3072;
 constexpr int kItemCost = 3, kGatedItemCost = 5;
 constexpr int kHalf = kTile / 2;  // scores of a row that one thread takes
 constexpr float kLazy = 8.0f;  // log2 of how far the maximum may pass its reference
+// log2 of the factor on a row's weights, in P, its sum and O alike: f16's largest power of two is 2^15.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 15.0f - kLazy : 0.0f;
+// A row's lse from its reference and its sum, which carries the factor (a power of two: exact).
+template <typename T>
+__device__ __forceinline__ float lse_of(float top, float scale, float sum) {
+    constexpr float kDrop = std::is_same<T, __half>::value ? 1.0f / 128.0f : 1.0f;
+    static_assert(kDrop * (1 << static_cast<int>(kLift<T>)) == 1.0f, "the factor and its inverse");
+    return sum == 0.f ? -INFINITY : top * scale + logf(sum * kDrop);
+}
 
 struct AttnParams {
     int H, KVH, D, G;
@@ -318,7 +332,7 @@ __global__ void __launch_bounds__(kMergeThreads) attn_merge_kernel(const AttnPar
     float4 gate[2];
     if (p.gate) load_gate8(p, t, h, col8 * 8, gate);
     put8<T>(p, t, h, col8 * 8, o, sum == 0.f ? 0.f : 1.f / sum, gate);
-    if (col8 == 0 && p.lse) p.lse[static_cast<size_t>(t) * p.H + h] = sum == 0.f ? -INFINITY : top * p.scale + logf(sum);
+    if (col8 == 0 && p.lse) p.lse[static_cast<size_t>(t) * p.H + h] = lse_of<T>(top, p.scale, sum);
 }
 
 template <typename T, int NCH, int NQ, bool PAIR>
@@ -989,7 +1003,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ, PAIR>::kThreads, 1)
                             }
                         }
                     }
-                    const float neg = m == -INFINITY ? 0.f : -m * c;
+                    const float neg = m == -INFINITY ? 0.f : kLift<T> - m * c;
                     const float2 c2 = make_float2(c, c), neg2 = make_float2(neg, neg);
                     float2 l0 = make_float2(0.f, 0.f), l1 = make_float2(0.f, 0.f);
                     if (!take_turn()) break;
@@ -1060,7 +1074,7 @@ __global__ void __launch_bounds__(Plan<NCH, NQ, PAIR>::kThreads, 1)
                         give(col + kOut, gate[1]);
                     }
                     if (live && half == 0 && p.lse)
-                        p.lse[static_cast<size_t>(t) * p.H + h] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
+                        p.lse[static_cast<size_t>(t) * p.H + h] = lse_of<T>(m, p.scale, l);
                 }
             } else if (any_live) {
                 // a shared item: this CTA's part (neighbouring rows' 16 bytes lie side by side)

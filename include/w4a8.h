@@ -408,6 +408,17 @@ W4A8_API w4a8_status w4a8_kv_evict(void* k, void* v, int32_t dtype, int32_t page
                                    const float* acc, const uint32_t* pos, int32_t stride, const uint32_t* keep,
                                    const uint32_t* protect_from, int32_t sink, float* acc_out, uint32_t* pos_out,
                                    uint32_t* len_out, void* workspace, size_t workspace_bytes, void* stream);
+/* The same for limits in two's complement, as a host with signed 32-bit arrays computes them: a
+ * protect_from at or below zero (seen - window of a sequence shorter than its window) protects
+ * every slot, a keep below zero keeps none.  w4a8_kv_evict takes such entries as values from 2^31
+ * on, which protect nothing and keep everything. */
+W4A8_API w4a8_status w4a8_kv_evict_signed(void* k, void* v, int32_t dtype, int32_t pages, int32_t page,
+                                          size_t page_stride, int32_t head_stride, int32_t row_stride, int32_t KVH,
+                                          int32_t D, const uint32_t* kv_len, const uint32_t* table, int32_t batch,
+                                          int32_t table_stride, const float* acc, const uint32_t* pos, int32_t stride,
+                                          const uint32_t* keep, const uint32_t* protect_from, int32_t sink,
+                                          float* acc_out, uint32_t* pos_out, uint32_t* len_out, void* workspace,
+                                          size_t workspace_bytes, void* stream);
 W4A8_API size_t w4a8_kv_evict_workspace_bytes(int32_t batch, int32_t KVH, int32_t stride);
 
 /* Index carried by a packed argmax key (0 for the "no value > -3e38" key 0). */

@@ -138,6 +138,13 @@ extern "C" {
                          stride: i32, keep: *const u32, protect_from: *const u32, sink: i32, acc_out: *mut f32,
                          pos_out: *mut u32, len_out: *mut u32, workspace: *mut c_void, workspace_bytes: usize,
                          stream: *mut c_void) -> w4a8_status;
+    pub fn w4a8_kv_evict_signed(k: *mut c_void, v: *mut c_void, dtype: i32, pages: i32, page: i32,
+                                page_stride: usize, head_stride: i32, row_stride: i32, kvh: i32, d: i32,
+                                kv_len: *const u32, table: *const u32, batch: i32, table_stride: i32,
+                                acc: *const f32, pos: *const u32, stride: i32, keep: *const u32,
+                                protect_from: *const u32, sink: i32, acc_out: *mut f32, pos_out: *mut u32,
+                                len_out: *mut u32, workspace: *mut c_void, workspace_bytes: usize,
+                                stream: *mut c_void) -> w4a8_status;
     pub fn w4a8_kv_evict_workspace_bytes(batch: i32, kvh: i32, stride: i32) -> usize;
     pub fn w4a8_group_dots(w: *const w4a8_weight, xq: *const i8, m: i32, dots: *mut i32,
                            stream: *mut c_void) -> w4a8_status;

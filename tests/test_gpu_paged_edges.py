@@ -2,12 +2,14 @@
 after their last MMA, long lines, tails of a softmax far below its largest weight, signed
 limits of the eviction, keys past shared memory."""
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 from oracle import paged as opg
-from webyiq_b200 import W4A8Error, ops
+from webyiq_b200 import W4A8Error, _lib, ops
 
 from test_gpu_paged import Case
 
@@ -110,3 +112,45 @@ def test_tail_beside_a_sink(cuda, lens, news, H, KVH, D, below):
     bad = (o.double() - ro).abs() > (2.0 ** -11 + 2e-5) * size + 2.0 ** -32 * 1.5 * many
     assert not bad.any(), (int(bad.sum()), ((o.double() - ro).abs() / ro.abs()).max().item())
     assert ((lse.double() - rl).abs() <= 1e-5 * (1 + rl.abs())).all()
+
+
+def _evicted(cuda, lens, keep, low, sink, acc, pos, seed=0):
+    """(positions kept of each head, len_out) of an eviction, checked against rows of the cache that moved with them."""
+    KVH, D = acc.shape[1], 64
+    c = Case(cuda, lens, [0] * len(lens), KVH, KVH, D, seed=seed)
+    k0 = c.host(c.k)
+    a, p, n = ops.kv_evict(c.kv, c.batch, torch.from_numpy(acc).to(cuda), c.i32(pos), c.i32(keep), c.i32(low), sink=sink)
+    p, n, k1 = p.cpu().numpy(), n.cpu().tolist(), c.host(c.k)
+    for b, L in enumerate(lens):
+        pg, row = opg.slots(c.table, b, L, c.page)
+        for h in range(KVH):
+            slot_of = {x: j for j, x in enumerate(pos[b, h, :L])}
+            came = [slot_of[x] for x in p[b, h, :n[b]]]
+            np.testing.assert_array_equal(k1[pg[:n[b]], h, row[:n[b]]], k0[pg[came], h, row[came]])
+    return [[sorted(p[b, h, :n[b]].tolist()) for h in range(KVH)] for b in range(len(lens))], n
+
+
+def test_evict_limits_are_signed(cuda):
+    """protect_from at or below zero protects every slot (a sequence shorter than its window of latest tokens),
+    so the lowest slots stay; a negative keep keeps none."""
+    rng = np.random.default_rng(1)
+    acc = rng.random((4, 2, 100)).astype(np.float32)
+    pos = np.stack([[rng.permutation(100) for _ in range(2)] for _ in range(4)])
+    kept, n = _evicted(cuda, [100] * 4, [40, 40, -3, 40], [-28, 0, 50, 2 ** 31 - 1], 0, acc, pos)
+    assert n == [40, 40, 0, 40]
+    for b in (0, 1):
+        assert kept[b] == [sorted(pos[b, h, :40].tolist()) for h in range(2)]
+    # protect_from past every position: by weight alone
+    assert kept[3] == [sorted(pos[3, h, np.argsort(-acc[3, h], kind="stable")[:40]].tolist()) for h in range(2)]
+    # the unsigned entry point takes the same bits as large values: nothing protected, everything kept
+    c = Case(cuda, [100] * 4, [0] * 4, 2, 2, 64)
+    dacc, dpos, n = torch.from_numpy(acc).to(cuda), c.i32(pos), torch.zeros(4, dtype=torch.int32, device=cuda)
+    ws = ops.kv_evict_workspace(c.batch, 2, cuda, 100)
+    keep, low = c.i32([40, 40, -3, 40]), c.i32([-28, 0, 50, 2 ** 31 - 1])
+    p = [ctypes.c_void_p(t.data_ptr()) for t in (c.k, c.v, c.batch.kv_len, c.batch.table, dacc, dpos, keep, low, n, ws)]
+    st = _lib.load().w4a8_kv_evict(p[0], p[1], *c.kv.layout, 2, 64, p[2], p[3], 4, c.batch.table.shape[1], p[4], p[5], 100,
+                                   p[6], p[7], 0, p[4], p[5], p[8], p[9], ws.numel(), None)
+    torch.cuda.synchronize()
+    assert st == _lib.OK and n.cpu().tolist() == [40, 40, 100, 40]
+    got = sorted(dpos[0, 0, :40].cpu().tolist())
+    assert got == sorted(pos[0, 0, np.argsort(-acc[0, 0], kind="stable")[:40]].tolist())

@@ -70,6 +70,8 @@ _SIGS = {
     "w4a8_attn_weights_workspace_bytes": (ctypes.c_size_t, [_I, _I, _I]),
     "w4a8_kv_evict": (ctypes.c_int, [_P, _P, _I, _I, _I, ctypes.c_size_t, _I, _I, _I, _I, _P, _P, _I, _I, _P, _P,
                                      _I, _P, _P, _I, _P, _P, _P, _P, ctypes.c_size_t, _P]),
+    "w4a8_kv_evict_signed": (ctypes.c_int, [_P, _P, _I, _I, _I, ctypes.c_size_t, _I, _I, _I, _I, _P, _P, _I, _I, _P, _P,
+                                            _I, _P, _P, _I, _P, _P, _P, _P, ctypes.c_size_t, _P]),
     "w4a8_kv_evict_workspace_bytes": (ctypes.c_size_t, [_I, _I, _I]),
     "w4a8_nccl_get_unique_id": (ctypes.c_int, [_P]),
     "w4a8_nccl_comm_init": (ctypes.c_int, [_I, _P, _I, ctypes.POINTER(ctypes.c_void_p)]),

@@ -41,6 +41,7 @@ struct EvictParams {
     int stride;  // slots of a row of acc and pos, in and out
     const uint32_t* keep;
     const uint32_t* protect_from;
+    bool limits_signed;  // keep and protect_from are two's complement, below zero as zero
     int sink;
     float* acc_out;
     uint32_t* pos_out;
@@ -52,6 +53,12 @@ struct EvictParams {
     PagedCache c;
     PagedBatch b;
 };
+
+// An entry of keep or protect_from.
+__device__ __forceinline__ uint32_t limit_of(const EvictParams& p, const uint32_t* at) {
+    const uint32_t x = ld_dep(at);
+    return p.limits_signed ? static_cast<uint32_t>(max(static_cast<int>(x), 0)) : x;
+}
 
 // Unsigned key in the order of the ranking: larger stays longer.
 __device__ __forceinline__ uint32_t rank_key(float w, uint32_t pos, int sink, uint32_t protect_from) {
@@ -99,8 +106,8 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
     const uint32_t cap = min(static_cast<uint32_t>(p.b.table_stride) * static_cast<uint32_t>(p.c.page),
                              static_cast<uint32_t>(p.stride));
     const int len = static_cast<int>(min(ld_dep(p.b.kv_len + seq), cap));
-    const int n = static_cast<int>(min(static_cast<uint32_t>(len), ld_dep(p.keep + seq)));
-    const uint32_t from = ld_dep(p.protect_from + seq);
+    const int n = static_cast<int>(min(static_cast<uint32_t>(len), limit_of(p, p.keep + seq)));
+    const uint32_t from = limit_of(p, p.protect_from + seq);
     const size_t row = static_cast<size_t>(seq) * p.KVH + kh;
     const float* acc = p.acc + row * p.stride;
     const uint32_t* pos = p.pos + row * p.stride;
@@ -292,27 +299,22 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
 
 int sm_count();  // capi.cu
 
-}  // namespace w4a8
+namespace {
 
-using namespace w4a8;
-
-extern "C" {
-
-W4A8_API size_t w4a8_kv_evict_workspace_bytes(int32_t batch, int32_t KVH, int32_t stride) {
+size_t workspace_of(int batch, int KVH, int stride) {
     if (batch < 1 || KVH < 1 || stride < 1) return 0;
     const size_t rows = static_cast<size_t>(batch) * KVH;
     const size_t moves = rows * 2 * (static_cast<size_t>(stride) / 2 + 1) * 4;
     return (rows * 4 + 255) / 256 * 256 + (moves + 255) / 256 * 256 + (stride > kSharedKeys ? rows * stride * 4 : 0);
 }
 
-W4A8_API w4a8_status w4a8_kv_evict(void* k, void* v, int32_t dtype, int32_t pages, int32_t page, size_t page_stride,
-                                   int32_t head_stride, int32_t row_stride, int32_t KVH, int32_t D,
-                                   const uint32_t* kv_len, const uint32_t* table, int32_t batch, int32_t table_stride,
-                                   const float* acc, const uint32_t* pos, int32_t stride, const uint32_t* keep,
-                                   const uint32_t* protect_from, int32_t sink, float* acc_out, uint32_t* pos_out,
-                                   uint32_t* len_out, void* workspace, size_t workspace_bytes, void* stream) {
-    const char* what = "w4a8_kv_evict";
+w4a8_status evict(const char* what, bool limits_signed, void* k, void* v, int dtype, int pages, int page, size_t page_stride,
+                  int head_stride, int row_stride, int KVH, int D, const uint32_t* kv_len, const uint32_t* table, int batch,
+                  int table_stride, const float* acc, const uint32_t* pos, int stride, const uint32_t* keep,
+                  const uint32_t* protect_from, int sink, float* acc_out, uint32_t* pos_out, uint32_t* len_out,
+                  void* workspace, size_t workspace_bytes, void* stream) {
     EvictParams p{};
+    p.limits_signed = limits_signed;
     p.c = PagedCache{k, v, dtype, pages, page, page_stride, head_stride, row_stride};
     // no new tokens here: kv_len stands in for the starts, which no kernel below reads
     p.b = PagedBatch{kv_len, kv_len, table, batch, table_stride, 0};
@@ -328,7 +330,7 @@ W4A8_API w4a8_status w4a8_kv_evict(void* k, void* v, int32_t dtype, int32_t page
     if (len_out == kv_len) return set_error(W4A8_EINVAL, "%s: len_out is kv_len (each head's CTA reads it)", what);
     if (static_cast<long long>(batch) * KVH > 65535)
         return set_error(W4A8_EINVAL, "%s: %d sequences of %d heads (at most 65535 in all)", what, batch, KVH);
-    if (!workspace || !aligned(workspace, 16) || workspace_bytes < w4a8_kv_evict_workspace_bytes(batch, KVH, stride))
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < workspace_of(batch, KVH, stride))
         return set_error(W4A8_EINVAL, "%s: workspace NULL, small or misaligned", what);
     p.KVH = KVH;
     p.D = D;
@@ -364,6 +366,41 @@ W4A8_API w4a8_status w4a8_kv_evict(void* k, void* v, int32_t dtype, int32_t page
     per = std::min<long long>(per, (most + kMoveThreads - 1) / kMoveThreads);
     return launch_pdl(what, evict_move_kernel, dim3(static_cast<unsigned>(per), static_cast<unsigned>(rows)),
                       dim3(kMoveThreads), 0, cs, p);
+}
+
+}  // namespace
+
+}  // namespace w4a8
+
+using namespace w4a8;
+
+extern "C" {
+
+W4A8_API size_t w4a8_kv_evict_workspace_bytes(int32_t batch, int32_t KVH, int32_t stride) {
+    return workspace_of(batch, KVH, stride);
+}
+
+W4A8_API w4a8_status w4a8_kv_evict(void* k, void* v, int32_t dtype, int32_t pages, int32_t page, size_t page_stride,
+                                   int32_t head_stride, int32_t row_stride, int32_t KVH, int32_t D,
+                                   const uint32_t* kv_len, const uint32_t* table, int32_t batch, int32_t table_stride,
+                                   const float* acc, const uint32_t* pos, int32_t stride, const uint32_t* keep,
+                                   const uint32_t* protect_from, int32_t sink, float* acc_out, uint32_t* pos_out,
+                                   uint32_t* len_out, void* workspace, size_t workspace_bytes, void* stream) {
+    return evict("w4a8_kv_evict", false, k, v, dtype, pages, page, page_stride, head_stride, row_stride, KVH, D, kv_len, table,
+                 batch, table_stride, acc, pos, stride, keep, protect_from, sink, acc_out, pos_out, len_out, workspace,
+                 workspace_bytes, stream);
+}
+
+W4A8_API w4a8_status w4a8_kv_evict_signed(void* k, void* v, int32_t dtype, int32_t pages, int32_t page, size_t page_stride,
+                                          int32_t head_stride, int32_t row_stride, int32_t KVH, int32_t D,
+                                          const uint32_t* kv_len, const uint32_t* table, int32_t batch,
+                                          int32_t table_stride, const float* acc, const uint32_t* pos, int32_t stride,
+                                          const uint32_t* keep, const uint32_t* protect_from, int32_t sink, float* acc_out,
+                                          uint32_t* pos_out, uint32_t* len_out, void* workspace, size_t workspace_bytes,
+                                          void* stream) {
+    return evict("w4a8_kv_evict_signed", true, k, v, dtype, pages, page, page_stride, head_stride, row_stride, KVH, D, kv_len,
+                 table, batch, table_stride, acc, pos, stride, keep, protect_from, sink, acc_out, pos_out, len_out, workspace,
+                 workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -486,7 +486,8 @@ def kv_evict_workspace(batch, KVH, device, slots=None):
 
 def kv_evict(kv, batch, acc, pos, keep, protect_from, sink=0, acc_out=None, pos_out=None, len_out=None, workspace=None):
     """Eviction by accumulated weight (w4a8.h): of each sequence's slots keep[b] (int32) stay,
-    in place in the cache; acc f32 and pos int32 [B, KVH, slots].  Returns (acc_out, pos_out,
+    in place in the cache; acc f32 and pos int32 [B, KVH, slots].  protect_from int32 [B]: the slots
+    of positions from there on are protected (all where it is 0 or less).  Returns (acc_out, pos_out,
     len_out): acc_out and pos_out default to acc and pos themselves, len_out to a new tensor
     (it may not be batch.kv_len)."""
     shape = acc.shape
@@ -513,7 +514,7 @@ def kv_evict(kv, batch, acc, pos, keep, protect_from, sink=0, acc_out=None, pos_
         workspace = kv_evict_workspace(batch, kv.KVH, kv.device, slots)
     elif not _is(workspace, torch.uint8):
         raise ValueError("kv_evict: workspace uint8")
-    st = _lib.load().w4a8_kv_evict(
+    st = _lib.load().w4a8_kv_evict_signed(
         kv.pk, kv.pv, *kv.layout, kv.KVH, kv.D, batch.pl, batch.pt, batch.B, batch.per, acc.data_ptr(), pos.data_ptr(),
         slots, keep.data_ptr(), protect_from.data_ptr(), sink, acc_out.data_ptr(), pos_out.data_ptr(), len_out.data_ptr(),
         workspace.data_ptr(), workspace.numel(), _raw_stream(kv.device))

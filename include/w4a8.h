@@ -392,8 +392,9 @@ W4A8_API w4a8_status w4a8_attn_weights(const void* q, int32_t q_row_stride, cons
 W4A8_API size_t w4a8_attn_weights_workspace_bytes(int32_t H, int32_t KVH, int32_t max_q);
 
 /* Eviction by accumulated weight, for each sequence and kv head on its own: of len =
- * kv_len[b] slots the n = min(len, keep[b]) stay that come first by (protected, weight
- * acc, lower slot), NaN ranking as the lowest weight; a slot is protected where its
+ * kv_len[b] slots the n = min(len, keep[b]) stay that come first: the
+ * protected ones by slot, the lower first, then by weight acc, the larger first (the lower
+ * slot among equals; NaN ranks as the lowest weight, and +inf protects nothing); a slot is protected where its
  * token's position pos (u32[batch, KVH, stride], as acc) is below sink or at least
  * protect_from[b].  The i-th kept slot at n or past it moves into the i-th dropped slot
  * below n, K and V rows, weight and position; every other slot stays where it is

@@ -83,9 +83,9 @@ def evict(k, v, table, kv_len, acc, pos, keep, protect_from, sink):
         pg, row = slots(table, b, L, page)
         for h in range(k.shape[1]):
             a, p = acc[b, h, :L], pos[b, h, :L]
-            w = [np.inf if p[j] < sink or p[j] >= protect_from[b] else (-np.inf if np.isnan(a[j]) else a[j])
-                 for j in range(L)]
-            kept = set(sorted(range(L), key=lambda j: (-w[j], j))[:n])
+            safe = [p[j] < sink or p[j] >= protect_from[b] for j in range(L)]  # before any weight, by slot
+            w = [0.0 if safe[j] else (-np.inf if np.isnan(a[j]) else a[j]) for j in range(L)]
+            kept = set(sorted(range(L), key=lambda j: (not safe[j], -w[j], j))[:n])
             came = np.arange(n)
             came[[j for j in range(n) if j not in kept]] = sorted(j for j in kept if j >= n)
             for x in (k, v):

@@ -154,3 +154,15 @@ def test_evict_limits_are_signed(cuda):
     assert st == _lib.OK and n.cpu().tolist() == [40, 40, 100, 40]
     got = sorted(dpos[0, 0, :40].cpu().tolist())
     assert got == sorted(pos[0, 0, np.argsort(-acc[0, 0], kind="stable")[:40]].tolist())
+
+
+def test_evict_infinite_weight_is_no_protection(cuda):
+    """Protected slots come before any weight, +inf too, whatever the slots' order."""
+    acc = np.ones((1, 2, 64), np.float32)
+    acc[0, 0, :30] = np.inf
+    acc[0, 1, 3:50:2] = np.inf
+    pos = np.tile(np.arange(64), (1, 2, 1))
+    kept, n = _evicted(cuda, [64], [16], [56], 4, acc, pos)
+    assert n == [16]
+    assert kept[0][0] == [*range(8), *range(56, 64)]                         # 4 sinks, the first 4 infinite, the latest 8
+    assert kept[0][1] == [0, 1, 2, 3, 5, 7, 9, 11, *range(56, 64)]

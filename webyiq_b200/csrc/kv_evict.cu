@@ -1,9 +1,9 @@
 // Eviction from the paged cache by accumulated attention weight.
 //
 // Per sequence and kv head, of `len` slots the n = min(len, keep) first of this order
-// stay: the protected ones (position below `sink`, or from protect_from on), then by
-// weight, largest first, the lower slot first among equals.  A weight of NaN ranks
-// as the lowest value.  The kept slots that lie at n or past it move into the slots
+// stay: the protected ones (position below `sink`, or from protect_from on), the lower
+// slot first, then by weight, largest first, the lower slot first among equals.  A weight
+// of NaN ranks as the lowest value, +inf below the protected ones.  The kept slots that lie at n or past it move into the slots
 // below n that were dropped, the i-th into the i-th: keys carry their rotation, so
 // a slot's place does not matter, and nothing else has to move.  Sources lie at n or
 // past it and destinations below n, so the moves are independent of one another.
@@ -62,7 +62,7 @@ __device__ __forceinline__ uint32_t limit_of(const EvictParams& p, const uint32_
 
 // Unsigned key in the order of the ranking: larger stays longer.
 __device__ __forceinline__ uint32_t rank_key(float w, uint32_t pos, int sink, uint32_t protect_from) {
-    if (pos < static_cast<uint32_t>(sink) || pos >= protect_from) return 0xff800000u;  // +inf's key
+    if (pos < static_cast<uint32_t>(sink) || pos >= protect_from) return 0xffffffffu;  // past +inf's key, 0xff800000
     if (w != w) return 0x007fffffu;                                                     // -inf's key
     const uint32_t u = __float_as_uint(w == 0.f ? 0.f : w);
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);

@@ -11,7 +11,7 @@ import torch
 from oracle import paged as opg
 from webyiq_b200 import W4A8Error, _lib, ops
 
-from test_gpu_paged import Case
+from test_gpu_paged import Case, test_evict as check_evict
 
 pytestmark = pytest.mark.gpu
 
@@ -166,3 +166,17 @@ def test_evict_infinite_weight_is_no_protection(cuda):
     assert n == [16]
     assert kept[0][0] == [*range(8), *range(56, 64)]                         # 4 sinks, the first 4 infinite, the latest 8
     assert kept[0][1] == [0, 1, 2, 3, 5, 7, 9, 11, *range(56, 64)]
+
+
+@pytest.mark.parametrize("stride,kind,dtype", [(49152, "ties", "f16"), (49153, "ties", "f16"), (49153, "odd", "bf16"),
+                                               (70000, "spread", "bf16"), (70000, "ties", "f16")])
+def test_evict_keys_in_the_workspace(cuda, stride, kind, dtype):
+    """So many heads that each gets one CTA, whose keys lie in shared memory up to 49152 slots of a head and in the
+    workspace past that: both sides of it, with a separate output and in place."""
+    B, KVH = 26, 3
+    assert B * KVH * 2 > torch.cuda.get_device_properties(cuda).multi_processor_count  # (no clusters)
+    big = torch.zeros((B, KVH, stride), dtype=torch.float32, device=cuda)
+    keys = _lib.load().w4a8_kv_evict_workspace_bytes(B, KVH, stride) - 2 * B * KVH * (stride // 2 + 1) * 4
+    assert (keys >= big.numel() * 4) == (stride > 49152)
+    lens = [stride - 3, 20011] + [20 + b for b in range(B - 2)]  # (the helper's weights have three slots more)
+    check_evict(cuda, KVH, 16, 16, lens, [20001, 20000] + [13] * (B - 2), kind, dtype)

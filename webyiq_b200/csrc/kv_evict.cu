@@ -9,7 +9,7 @@
 // past it and destinations below n, so the moves are independent of one another.
 //
 // A cluster of 1 to 8 CTAs takes a (sequence, kv head), a stretch of the slots each: the keys
-// are read once into shared memory (51200 of them a CTA, in the workspace past that), the
+// are read once into shared memory (49152 of them a CTA, in the workspace past that), the
 // n-th largest is found from histograms of 11, 11 and 10 bits that the CTAs add up over
 // distributed shared memory.  Then each thread walks consecutive slots of its CTA's
 // stretch, and block-wide prefix sums, offset by the counts of the CTAs before, number the

@@ -400,7 +400,7 @@ W4A8_API size_t w4a8_attn_weights_workspace_bytes(int32_t H, int32_t KVH, int32_
  * below n, K and V rows, weight and position; every other slot stays where it is
  * (keys carry their rotation, so the order of slots has no meaning).  acc_out and pos_out
  * get the first n entries of each head (they may be acc and pos); len_out[b] = n
- * (not kv_len itself).  stride >= any kv_len.
+ * (not kv_len itself; keep or protect_from will do).  stride >= any kv_len.
  * workspace: w4a8_kv_evict_workspace_bytes(...) bytes, 16-byte aligned, any contents;
  * calls that share one must not overlap on the GPU. */
 W4A8_API w4a8_status w4a8_kv_evict(void* k, void* v, int32_t dtype, int32_t pages, int32_t page, size_t page_stride,

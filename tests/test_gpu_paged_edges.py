@@ -180,3 +180,23 @@ def test_evict_keys_in_the_workspace(cuda, stride, kind, dtype):
     assert (keys >= big.numel() * 4) == (stride > 49152)
     lens = [stride - 3, 20011] + [20 + b for b in range(B - 2)]  # (the helper's weights have three slots more)
     check_evict(cuda, KVH, 16, 16, lens, [20001, 20000] + [13] * (B - 2), kind, dtype)
+
+
+@pytest.mark.parametrize("over", ["keep", "low"])
+def test_evict_length_over_a_limit(cuda, over):
+    """len_out in the place of keep or of protect_from: every head still goes by the limits as they were."""
+    rng = np.random.default_rng(2)
+    B, KVH, L = 24, 16, 700
+    acc, pos = rng.random((B, KVH, L)).astype(np.float32), np.tile(np.arange(L), (B, KVH, 1))
+    for _ in range(5):
+        c = Case(cuda, [L] * B, [0] * B, KVH, KVH, 16)
+        limits = {"keep": c.i32([150 + b for b in range(B)]), "low": c.i32([L - 60 - b for b in range(B)])}
+        _, p, n = ops.kv_evict(c.kv, c.batch, torch.from_numpy(acc).to(cuda), c.i32(pos), limits["keep"], limits["low"],
+                               len_out=limits[over])
+        assert n is limits[over] and n.cpu().tolist() == [150 + b for b in range(B)]
+        p = p.cpu().numpy()
+        for b in range(B):
+            low = L - 60 - b
+            for h in range(KVH):
+                best = np.argsort(-acc[b, h, :low], kind="stable")[:150 + b - 60 - b]
+                assert sorted(p[b, h, :150 + b].tolist()) == sorted([*best.tolist(), *range(low, L)])

@@ -60,6 +60,16 @@ __device__ __forceinline__ uint32_t limit_of(const EvictParams& p, const uint32_
     return p.limits_signed ? static_cast<uint32_t>(max(static_cast<int>(x), 0)) : x;
 }
 
+// Slots of a sequence, as far as acc and pos reach, and how many of them stay.
+__device__ __forceinline__ int slots_of(const EvictParams& p, int seq) {
+    const uint32_t cap = min(static_cast<uint32_t>(p.b.table_stride) * static_cast<uint32_t>(p.c.page),
+                             static_cast<uint32_t>(p.stride));
+    return static_cast<int>(min(ld_dep(p.b.kv_len + seq), cap));
+}
+__device__ __forceinline__ int kept_of(const EvictParams& p, int seq, int len) {
+    return static_cast<int>(min(static_cast<uint32_t>(len), limit_of(p, p.keep + seq)));
+}
+
 // Unsigned key in the order of the ranking: larger stays longer.
 __device__ __forceinline__ uint32_t rank_key(float w, uint32_t pos, int sink, uint32_t protect_from) {
     if (pos < static_cast<uint32_t>(sink) || pos >= protect_from) return 0xffffffffu;  // past +inf's key, 0xff800000
@@ -103,17 +113,13 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
     const int kh = blockIdx.x / ctas, seq = blockIdx.y, tid = threadIdx.x;
-    const uint32_t cap = min(static_cast<uint32_t>(p.b.table_stride) * static_cast<uint32_t>(p.c.page),
-                             static_cast<uint32_t>(p.stride));
-    const int len = static_cast<int>(min(ld_dep(p.b.kv_len + seq), cap));
-    const int n = static_cast<int>(min(static_cast<uint32_t>(len), limit_of(p, p.keep + seq)));
+    const int len = slots_of(p, seq), n = kept_of(p, seq, len);
     const uint32_t from = limit_of(p, p.protect_from + seq);
     const size_t row = static_cast<size_t>(seq) * p.KVH + kh;
     const float* acc = p.acc + row * p.stride;
     const uint32_t* pos = p.pos + row * p.stride;
     float* acc_out = p.acc_out + row * p.stride;
     uint32_t* pos_out = p.pos_out + row * p.stride;
-    if (kh == 0 && rank == 0 && tid == 0) p.len_out[seq] = static_cast<uint32_t>(n);
     // this CTA's slots
     const int part = (len + ctas - 1) / ctas;
     const int s0 = min(rank * part, len), mine = min(part, len - s0);
@@ -272,6 +278,9 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
     pdl_launch_dependents();
     pdl_wait();
     const int seq = blockIdx.y / p.KVH, kh = blockIdx.y % p.KVH;
+    // the new length: here, where no CTA reads the batch's limits any more, so that it may take their place
+    if (kh == 0 && blockIdx.x == 0 && threadIdx.x == 0)
+        p.len_out[seq] = static_cast<uint32_t>(kept_of(p, seq, slots_of(p, seq)));
     const size_t row = blockIdx.y;
     const uint32_t count = ld_dep(p.count + row);
     const uint32_t* dst = p.moves + row * 2 * (p.stride / 2 + 1);
@@ -327,7 +336,7 @@ w4a8_status evict(const char* what, bool limits_signed, void* k, void* v, int dt
     if (!acc || !pos || !keep || !protect_from || !acc_out || !pos_out || !len_out)
         return set_error(W4A8_EINVAL, "%s: NULL pointer", what);
     if (stride < 1 || sink < 0) return set_error(W4A8_EINVAL, "%s: %d slots a head, sink %d", what, stride, sink);
-    if (len_out == kv_len) return set_error(W4A8_EINVAL, "%s: len_out is kv_len (each head's CTA reads it)", what);
+    if (len_out == kv_len) return set_error(W4A8_EINVAL, "%s: len_out is kv_len", what);
     if (static_cast<long long>(batch) * KVH > 65535)
         return set_error(W4A8_EINVAL, "%s: %d sequences of %d heads (at most 65535 in all)", what, batch, KVH);
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < workspace_of(batch, KVH, stride))

@@ -311,7 +311,7 @@ class PagedKV:
             raise ValueError("PagedKV takes k and v of the same strides, with inner stride 1")
         self.k, self.v = k, v
         self.pages, self.KVH, self.page, self.D = k.shape
-        self.dtype, self.device = k.dtype, k.device
+        self.dtype, self.device, self.index = k.dtype, k.device, k.get_device()
         self.scale = 1.0 / math.sqrt(self.D)  # of the scores, where a call gives none
         self.layout = (_TYPES[k.dtype], self.pages, self.page, k.stride(0), k.stride(1), k.stride(2))
         self.pk, self.pv = k.data_ptr(), v.data_ptr()
@@ -328,6 +328,9 @@ class PagedBatch:
 
     def __init__(self, q_start, kv_len, table, max_q, max_kv):
         _need_cuda(q_start, kv_len, table)
+        self.index = q_start.get_device()
+        if kv_len.get_device() != self.index or table.get_device() != self.index:
+            raise ValueError("PagedBatch takes tensors of one device")
         self.B = kv_len.numel()
         if q_start.dtype != torch.int32 or kv_len.dtype != torch.int32 or table.dtype != torch.int32:
             raise ValueError("PagedBatch takes int32 tensors")
@@ -343,27 +346,39 @@ class PagedBatch:
 # checks: each attribute of a tensor costs about a tenth of a microsecond.
 
 
-def _raw_stream(device):
+def _raw_stream(index):
     """The current stream of a device as an integer (torch.cuda.current_stream builds an object: 3 us)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
-def _is(t, dtype):
-    return t.dtype is dtype and t.is_cuda and t.is_contiguous()
+def _current_device():
+    return torch._C._cuda_getDevice()
 
 
-def _opt(t, dtype, what):
-    """Pointer of an optional contiguous CUDA tensor (0 for None)."""
+def _place(kv, batch):
+    """Before a call: the library launches on the current device, so everything has to be there."""
+    if batch.index != kv.index:
+        raise ValueError(f"a batch of cuda:{batch.index} with a cache of cuda:{kv.index}")
+    if _current_device() != kv.index:
+        raise ValueError(f"a cache of cuda:{kv.index}, which is not the current device")
+
+
+def _is(t, dtype, index):
+    return t.dtype is dtype and t.get_device() == index and t.is_contiguous()
+
+
+def _opt(t, dtype, what, index):
+    """Pointer of an optional contiguous tensor of a CUDA device (0 for None)."""
     if t is None:
         return 0
-    if not _is(t, dtype):
-        raise ValueError(f"{what}: a contiguous CUDA tensor of {dtype}")
+    if not _is(t, dtype, index):
+        raise ValueError(f"{what}: a contiguous tensor of {dtype} on cuda:{index}")
     return t.data_ptr()
 
 
 def _token_stride(name, t, kv):
     """Elements from token to token of a [tokens, heads, D] tensor of the cache's type, contiguous within a token."""
-    if t.dtype is not kv.dtype or t.device != kv.device or t.dim() != 3:
+    if t.dtype is not kv.dtype or t.get_device() != kv.index or t.dim() != 3:
         raise ValueError(f"{name}: a [tokens, heads, D] tensor of {kv.dtype} on {kv.device}")
     T, H, D = t.shape
     if D != kv.D:
@@ -381,7 +396,9 @@ def qk_norm_rope_kv(qkv, kv, batch, pos, rope, H, q_norm=None, k_norm=None, eps=
     heads of D in their place); pos int32 [tokens]; rope f32 [rows, rot] (cosines, then
     sines) or None; q_norm, k_norm f32 [D] or None.  Returns q [tokens, H, D] of the
     cache's type."""
-    if qkv.dtype is not torch.float32 or qkv.device != kv.device or qkv.dim() != 2:
+    _place(kv, batch)
+    at = kv.index
+    if qkv.dtype is not torch.float32 or qkv.get_device() != at or qkv.dim() != 2:
         raise ValueError(f"qk_norm_rope_kv: qkv f32 [tokens, heads * D] on {kv.device}")
     T, width = qkv.shape
     D = kv.D
@@ -389,23 +406,22 @@ def qk_norm_rope_kv(qkv, kv, batch, pos, rope, H, q_norm=None, k_norm=None, eps=
     row, inner = qkv.stride()
     if width != H * qhs + 2 * kv.KVH * D or (inner != 1 and T):
         raise ValueError(f"qk_norm_rope_kv: rows of {width} for {H} query and {kv.KVH} kv heads of {D}, inner stride 1")
-    pqn, pkn = _opt(q_norm, torch.float32, "q_norm"), _opt(k_norm, torch.float32, "k_norm")
+    pqn, pkn = _opt(q_norm, torch.float32, "q_norm", at), _opt(k_norm, torch.float32, "k_norm", at)
     if (pqn and q_norm.numel() != D) or (pkn and k_norm.numel() != D):
         raise ValueError("qk_norm_rope_kv: norm weights f32 [D]")
     rot = rows = prope = ppos = 0
     if rope is not None:
-        prope, ppos = _opt(rope, torch.float32, "rope"), _opt(pos, torch.int32, "pos")
+        prope, ppos = _opt(rope, torch.float32, "rope", at), _opt(pos, torch.int32, "pos", at)
         if rope.dim() != 2 or not ppos and T or ppos and pos.numel() != T:
             raise ValueError("qk_norm_rope_kv: rope f32 [rows, rot] and pos int32 [tokens]")
         rows, rot = rope.shape
     if q is None:
         q = torch.empty((T, H, D), dtype=kv.dtype, device=qkv.device)
-    elif q.shape != (T, H, D) or not _is(q, kv.dtype):
+    elif q.shape != (T, H, D) or not _is(q, kv.dtype, at):
         raise ValueError("qk_norm_rope_kv: q [tokens, H, D] of the cache's type, contiguous")
     st = _lib.load().w4a8_qk_norm_rope_kv(
         qkv.data_ptr(), row if T > 1 else width, qhs, H, kv.KVH, D, pqn, pkn, eps, prope, rot, rows, interleaved, ppos,
-        batch.pq, batch.pl, batch.pt, batch.B, batch.per, T, q.data_ptr(), kv.pk, kv.pv, *kv.layout,
-        _raw_stream(kv.device))
+        batch.pq, batch.pl, batch.pt, batch.B, batch.per, T, q.data_ptr(), kv.pk, kv.pv, *kv.layout, _raw_stream(at))
     if st:
         _lib.check(st)
     return q
@@ -422,30 +438,32 @@ def attn_paged(q, kv, batch, scale=None, gate=None, o=None, lse=None, workspace=
     type -> (o [tokens, H, D], lse f32 [tokens, H]); o of the cache's type, or f32 where
     an f32 o is given; gate f32 [tokens, H, D] (any token and head stride): o times
     sigmoid(gate).  scale defaults to 1 / sqrt(D)."""
+    _place(kv, batch)
+    at = kv.index
     row = _token_stride("attn_paged: q", q, kv)
     T, H, D = q.shape
     if o is None:
         o = torch.empty((T, H, D), dtype=kv.dtype, device=kv.device)
-    elif o.shape != q.shape or not (o.is_cuda and o.is_contiguous()):
+    elif o.shape != q.shape or not (o.get_device() == at and o.is_contiguous()):
         raise ValueError("attn_paged: o [tokens, H, D], contiguous")
     if lse is None:
         lse = torch.empty((T, H), dtype=torch.float32, device=kv.device)
-    elif lse.numel() != T * H or not _is(lse, torch.float32):
+    elif lse.numel() != T * H or not _is(lse, torch.float32, at):
         raise ValueError("attn_paged: lse f32 [tokens, H], contiguous")
     pg = gr = gh = 0
     if gate is not None:
         gs = gate.stride()
-        if gate.dtype is not torch.float32 or gate.shape != q.shape or gate.device != kv.device or gs[2] != 1:
+        if gate.dtype is not torch.float32 or gate.shape != q.shape or gate.get_device() != at or gs[2] != 1:
             raise ValueError("attn_paged: gate f32 [tokens, H, D] with inner stride 1")
         pg, gr, gh = gate.data_ptr(), gs[0], gs[1]
     if workspace is None:
         workspace = attn_paged_workspace(batch, T, H, kv.KVH, D, kv.device)
-    elif not _is(workspace, torch.uint8):
+    elif not _is(workspace, torch.uint8, at):
         raise ValueError("attn_paged: workspace uint8")
     st = _lib.load().w4a8_attn_paged(
         q.data_ptr(), row, H, kv.KVH, D, kv.scale if scale is None else scale, pg, gr, gh, batch.pq, batch.pl, batch.pt,
         batch.B, batch.per, T, batch.max_q, batch.max_kv, kv.pk, kv.pv, *kv.layout, o.data_ptr(), _TYPES.get(o.dtype, -1),
-        lse.data_ptr(), workspace.data_ptr(), workspace.numel(), _raw_stream(kv.device))
+        lse.data_ptr(), workspace.data_ptr(), workspace.numel(), _raw_stream(at))
     if st:
         _lib.check(st)
     return o, lse
@@ -460,18 +478,20 @@ def attn_weights_workspace(batch, H, KVH, device):
 def attn_weights(q, lse, kv, batch, acc, scale=None, workspace=None):
     """acc f32 [B, KVH, slots] += the attention weight each slot received from the new
     tokens (w4a8.h), with attn_paged's q, lse and scale.  Returns acc."""
+    _place(kv, batch)
+    at = kv.index
     row = _token_stride("attn_weights: q", q, kv)
     T, H, D = q.shape
-    if lse.numel() != T * H or not (_is(lse, torch.float32) or not T):
+    if lse.numel() != T * H or not (_is(lse, torch.float32, at) or not T):
         raise ValueError("attn_weights: lse f32 [tokens, H], contiguous")
-    if acc.dim() != 3 or acc.shape[0] != batch.B or acc.shape[1] != kv.KVH or not _is(acc, torch.float32):
+    if acc.dim() != 3 or acc.shape[0] != batch.B or acc.shape[1] != kv.KVH or not _is(acc, torch.float32, at):
         raise ValueError("attn_weights: acc f32 [B, KVH, slots], contiguous")
     if workspace is None:
         workspace = attn_weights_workspace(batch, H, kv.KVH, kv.device)
     st = _lib.load().w4a8_attn_weights(
         q.data_ptr(), row, lse.data_ptr(), H, kv.KVH, D, kv.scale if scale is None else scale, batch.pq, batch.pl, batch.pt,
         batch.B, batch.per, T, batch.max_q, batch.max_kv, kv.pk, *kv.layout, acc.data_ptr(), acc.shape[2],
-        _opt(workspace, torch.uint8, "workspace"), 0 if workspace is None else workspace.numel(), _raw_stream(kv.device))
+        _opt(workspace, torch.uint8, "workspace", at), 0 if workspace is None else workspace.numel(), _raw_stream(at))
     if st:
         _lib.check(st)
     return acc
@@ -490,34 +510,35 @@ def kv_evict(kv, batch, acc, pos, keep, protect_from, sink=0, acc_out=None, pos_
     of positions from there on are protected (all where it is 0 or less).  Returns (acc_out, pos_out,
     len_out): acc_out and pos_out default to acc and pos themselves, len_out to a new tensor
     (it may not be batch.kv_len)."""
-    shape = acc.shape
-    if len(shape) != 3 or shape[0] != batch.B or shape[1] != kv.KVH or not _is(acc, torch.float32) or \
-            pos.shape != shape or not _is(pos, torch.int32):
+    _place(kv, batch)
+    shape, at = acc.shape, kv.index
+    if len(shape) != 3 or shape[0] != batch.B or shape[1] != kv.KVH or not _is(acc, torch.float32, at) or \
+            pos.shape != shape or not _is(pos, torch.int32, at):
         raise ValueError("kv_evict: acc f32 and pos int32 [B, KVH, slots], contiguous")
     slots = shape[2]
     if slots < batch.max_kv:
         raise ValueError(f"kv_evict: {slots} weights a head for up to {batch.max_kv} slots")
     if acc_out is None:
         acc_out = acc
-    elif acc_out.shape != shape or not _is(acc_out, torch.float32):
+    elif acc_out.shape != shape or not _is(acc_out, torch.float32, at):
         raise ValueError("kv_evict: acc_out as acc")
     if pos_out is None:
         pos_out = pos
-    elif pos_out.shape != shape or not _is(pos_out, torch.int32):
+    elif pos_out.shape != shape or not _is(pos_out, torch.int32, at):
         raise ValueError("kv_evict: pos_out as pos")
     if len_out is None:
         len_out = torch.empty_like(batch.kv_len)
     for t in (keep, protect_from, len_out):
-        if t.numel() != batch.B or not _is(t, torch.int32):
+        if t.numel() != batch.B or not _is(t, torch.int32, at):
             raise ValueError("kv_evict: keep, protect_from and len_out int32 [B]")
     if workspace is None:
         workspace = kv_evict_workspace(batch, kv.KVH, kv.device, slots)
-    elif not _is(workspace, torch.uint8):
+    elif not _is(workspace, torch.uint8, at):
         raise ValueError("kv_evict: workspace uint8")
     st = _lib.load().w4a8_kv_evict_signed(
         kv.pk, kv.pv, *kv.layout, kv.KVH, kv.D, batch.pl, batch.pt, batch.B, batch.per, acc.data_ptr(), pos.data_ptr(),
         slots, keep.data_ptr(), protect_from.data_ptr(), sink, acc_out.data_ptr(), pos_out.data_ptr(), len_out.data_ptr(),
-        workspace.data_ptr(), workspace.numel(), _raw_stream(kv.device))
+        workspace.data_ptr(), workspace.numel(), _raw_stream(at))
     if st:
         _lib.check(st)
     return acc_out, pos_out, len_out

@@ -152,3 +152,36 @@ def test_refuses_another_device(lib, op):
     with pytest.raises(ValueError, match="current device"):
         call(op, tensors(op))
     assert not [c for c in lib.calls if c[0] == ENTRY[op]]
+
+
+@pytest.mark.parametrize("op", OWN)
+@pytest.mark.parametrize("name", SHAPES)
+def test_refuses_a_tensor_that_moved(lib, op, name):
+    """PagedKV and PagedBatch hold addresses: a tensor that was resized or set to other memory after they were made
+    leaves them behind, and nothing is launched on them."""
+    for moved in (name, "v") if name == "k" else (name,):
+        t = tensors(op)
+        kv, batch = ops.PagedKV(t["k"], t["v"]), ops.PagedBatch(t["q_start"], t["kv_len"], t["table"], 3, CAP)
+        invoke(op, t, kv, batch)
+        lib.calls.clear()
+        t[moved].ptr += 4096
+        with pytest.raises(ValueError, match="moved"):
+            invoke(op, t, kv, batch)
+        assert not lib.calls
+
+
+def test_attributes_that_are_fixed(lib):
+    """What a call would not notice cannot be assigned; the bounds and the scale, which it reads, can."""
+    t = tensors("attn")
+    kv, batch = ops.PagedKV(t["k"], t["v"]), ops.PagedBatch(t["q_start"], t["kv_len"], t["table"], 3, CAP)
+    for x, names in ((kv, ("k", "v", "pages", "page", "KVH", "D", "dtype", "device", "layout", "other")),
+                     (batch, ("q_start", "kv_len", "table", "B", "per", "other"))):
+        for name in names:
+            with pytest.raises(AttributeError):
+                setattr(x, name, getattr(x, name, 0))
+    assert kv.k is t["k"] and batch.kv_len is t["kv_len"]
+    batch.max_q, batch.max_kv, kv.scale = 7, 50, 0.25
+    lib.calls.clear()
+    invoke("attn", t, kv, batch)
+    (_, args), = lib.calls
+    assert args[5] == 0.25 and args[15:17] == (7, 50)

@@ -297,10 +297,24 @@ def deltanet(proj, conv_w, conv_state, state, neg_a, dt_bias, gate_norm, params,
 _TYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 
 
-class PagedKV:
+class _Fixed:
+    """Attributes that hold for the object's life, but those of `free`, which every call reads anew."""
+
+    free = ()
+
+    def __setattr__(self, name, value):
+        if name not in self.free:
+            raise AttributeError(f"{type(self).__name__}.{name} is fixed: make a new {type(self).__name__}")
+        self.__dict__[name] = value
+
+
+class PagedKV(_Fixed):
     """A paged KV cache in device memory: k, v [pages, KVH, page, D], f16 or bf16, of the
     same strides.  Any order of the dimensions in memory does (a cache stored [pages, page,
-    KVH, D] comes in as its permute(0, 2, 1, 3)); the inner stride is 1."""
+    KVH, D] comes in as its permute(0, 2, 1, 3)); the inner stride is 1.  It holds the tensors'
+    addresses: writing to them is fine, a tensor resized or set to other memory is refused."""
+
+    free = ("scale",)
 
     def __init__(self, k, v):
         if not (k.is_cuda and v.is_cuda) or k.device != v.device:
@@ -309,37 +323,40 @@ class PagedKV:
             raise ValueError("PagedKV takes k and v [pages, KVH, page, D] of one type, float16 or bfloat16")
         if k.stride() != v.stride() or k.stride(3) != 1:
             raise ValueError("PagedKV takes k and v of the same strides, with inner stride 1")
-        self.k, self.v = k, v
-        self.pages, self.KVH, self.page, self.D = k.shape
-        self.dtype, self.device, self.index = k.dtype, k.device, k.get_device()
-        self.scale = 1.0 / math.sqrt(self.D)  # of the scores, where a call gives none
-        self.layout = (_TYPES[k.dtype], self.pages, self.page, k.stride(0), k.stride(1), k.stride(2))
-        self.pk, self.pv = k.data_ptr(), v.data_ptr()
+        pages, KVH, page, D = k.shape
+        self.__dict__.update(
+            k=k, v=v, pages=pages, KVH=KVH, page=page, D=D, dtype=k.dtype, device=k.device, index=k.get_device(),
+            scale=1.0 / math.sqrt(D),  # of the scores, where a call gives none
+            layout=(_TYPES[k.dtype], pages, page, k.stride(0), k.stride(1), k.stride(2)),
+            pk=k.data_ptr(), pv=v.data_ptr(), at=(k.data_ptr(), v.data_ptr()), now=(k.data_ptr, v.data_ptr))
 
     def __repr__(self):
         return f"PagedKV(pages={self.pages}, KVH={self.KVH}, page={self.page}, D={self.D}, {self.dtype})"
 
 
-class PagedBatch:
+class PagedBatch(_Fixed):
     """A step's batch over a PagedKV: q_start int32 [B + 1] (first new token of each sequence,
     from 0), kv_len int32 [B] (slots, the new tokens' own among them), table int32 [B, pages a
     sequence].  max_q and max_kv bound the new tokens and the slots of any sequence (read on
-    the device otherwise, so the arrays may be rewritten in place between calls)."""
+    the device otherwise, so the arrays may be rewritten in place between calls); the two may
+    be assigned anew.  Holds the arrays' addresses, as PagedKV does."""
+
+    free = ("max_q", "max_kv")
 
     def __init__(self, q_start, kv_len, table, max_q, max_kv):
         _need_cuda(q_start, kv_len, table)
-        self.index = q_start.get_device()
-        if kv_len.get_device() != self.index or table.get_device() != self.index:
+        index, B = q_start.get_device(), kv_len.numel()
+        if kv_len.get_device() != index or table.get_device() != index:
             raise ValueError("PagedBatch takes tensors of one device")
-        self.B = kv_len.numel()
         if q_start.dtype != torch.int32 or kv_len.dtype != torch.int32 or table.dtype != torch.int32:
             raise ValueError("PagedBatch takes int32 tensors")
-        if q_start.numel() != self.B + 1 or table.dim() != 2 or table.shape[0] != self.B:
+        if q_start.numel() != B + 1 or table.dim() != 2 or table.shape[0] != B:
             raise ValueError("PagedBatch takes q_start [B + 1], kv_len [B] and table [B, pages a sequence]")
-        self.q_start, self.kv_len, self.table = q_start, kv_len, table
-        self.max_q, self.max_kv = int(max_q), int(max_kv)
-        self.per = table.shape[1]
-        self.pq, self.pl, self.pt = q_start.data_ptr(), kv_len.data_ptr(), table.data_ptr()
+        self.__dict__.update(
+            q_start=q_start, kv_len=kv_len, table=table, max_q=int(max_q), max_kv=int(max_kv), B=B, per=table.shape[1],
+            index=index, pq=q_start.data_ptr(), pl=kv_len.data_ptr(), pt=table.data_ptr(),
+            at=(q_start.data_ptr(), kv_len.data_ptr(), table.data_ptr()),
+            now=(q_start.data_ptr, kv_len.data_ptr, table.data_ptr))
 
 
 # The paged operators are called once a layer and token, so their wrappers keep to cheap
@@ -356,7 +373,12 @@ def _current_device():
 
 
 def _place(kv, batch):
-    """Before a call: the library launches on the current device, so everything has to be there."""
+    """Before a call: the library launches on the current device, so everything has to be there, and at the
+    addresses that were taken."""
+    k, v = kv.now
+    q_start, kv_len, table = batch.now
+    if (k(), v()) != kv.at or (q_start(), kv_len(), table()) != batch.at:
+        raise ValueError("the cache's or the batch's tensors have moved since PagedKV or PagedBatch took them")
     if batch.index != kv.index:
         raise ValueError(f"a batch of cuda:{batch.index} with a cache of cuda:{kv.index}")
     if _current_device() != kv.index:
@@ -371,7 +393,7 @@ def _opt(t, dtype, what, index):
     """Pointer of an optional contiguous tensor of a CUDA device (0 for None)."""
     if t is None:
         return 0
-    if not _is(t, dtype, index):
+    if t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():
         raise ValueError(f"{what}: a contiguous tensor of {dtype} on cuda:{index}")
     return t.data_ptr()
 
@@ -512,24 +534,22 @@ def kv_evict(kv, batch, acc, pos, keep, protect_from, sink=0, acc_out=None, pos_
     (it may not be batch.kv_len)."""
     _place(kv, batch)
     shape, at = acc.shape, kv.index
-    if len(shape) != 3 or shape[0] != batch.B or shape[1] != kv.KVH or not _is(acc, torch.float32, at) or \
-            pos.shape != shape or not _is(pos, torch.int32, at):
+    if len(shape) != 3 or shape[0] != batch.B or shape[1] != kv.KVH:
         raise ValueError("kv_evict: acc f32 and pos int32 [B, KVH, slots], contiguous")
     slots = shape[2]
     if slots < batch.max_kv:
         raise ValueError(f"kv_evict: {slots} weights a head for up to {batch.max_kv} slots")
     if acc_out is None:
         acc_out = acc
-    elif acc_out.shape != shape or not _is(acc_out, torch.float32, at):
-        raise ValueError("kv_evict: acc_out as acc")
     if pos_out is None:
         pos_out = pos
-    elif pos_out.shape != shape or not _is(pos_out, torch.int32, at):
-        raise ValueError("kv_evict: pos_out as pos")
     if len_out is None:
         len_out = torch.empty_like(batch.kv_len)
+    for t, dtype in ((acc, torch.float32), (pos, torch.int32), (acc_out, torch.float32), (pos_out, torch.int32)):
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != at or not t.is_contiguous():
+            raise ValueError("kv_evict: acc f32 and pos int32 [B, KVH, slots], contiguous; acc_out and pos_out as they")
     for t in (keep, protect_from, len_out):
-        if t.numel() != batch.B or not _is(t, torch.int32, at):
+        if t.dtype is not torch.int32 or t.numel() != batch.B or t.get_device() != at or not t.is_contiguous():
             raise ValueError("kv_evict: keep, protect_from and len_out int32 [B]")
     if workspace is None:
         workspace = kv_evict_workspace(batch, kv.KVH, kv.device, slots)

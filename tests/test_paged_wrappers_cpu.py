@@ -185,3 +185,42 @@ def test_attributes_that_are_fixed(lib):
     invoke("attn", t, kv, batch)
     (_, args), = lib.calls
     assert args[5] == 0.25 and args[15:17] == (7, 50)
+
+
+@pytest.mark.parametrize("op,name,stride", [
+    ("attn", "k", (2 ** 33, 2 ** 31, D, 1)), ("attn", "k", (2 ** 40, 2 ** 33, 2 ** 32 + D, 1)),
+    ("rope", "k", (PAGE * D, 2 ** 32 + PAGES * PAGE * D, D, 1)),  # heads outermost: cut to 32 bits it would still nest
+    ("attn", "q", (2 ** 32 + H * D, D, 1)), ("weights", "q", (2 ** 31, D, 1)), ("rope", "qkv", (2 ** 32 + 1024, 1)),
+    ("attn", "gate", (2 ** 32 + H * D, D, 1)), ("attn", "gate", (H * D, 2 ** 32 + D, 1))])
+def test_refuses_strides_past_31_bits(lib, op, name, stride):
+    """The library's strides but the pages' are 32-bit: a longer one would be cut to its low bits."""
+    t = tensors(op)
+    t[name].strides = stride
+    if name == "k":
+        t["v"].strides = stride
+    with pytest.raises(ValueError, match="2\\^31"):
+        call(op, t)
+    assert not [c for c in lib.calls if c[0] == ENTRY[op]]
+
+
+@pytest.mark.parametrize("bounds", [(2 ** 32, CAP), (2 ** 32 + 3, CAP), (3, 2 ** 32), (3, 2 ** 31), (-1, CAP)])
+def test_refuses_bounds_past_31_bits(lib, bounds):
+    """max_q = 2^32 would be 0 to the library: nothing computed and no error."""
+    t = tensors("weights")
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops.PagedBatch(t["q_start"], t["kv_len"], t["table"], *bounds)
+    batch = ops.PagedBatch(t["q_start"], t["kv_len"], t["table"], 3, CAP)
+    with pytest.raises(ValueError, match="2\\^31"):
+        batch.max_q, batch.max_kv = bounds
+
+
+def test_refuses_sizes_past_31_bits(lib):
+    t = tensors("attn", table=Fake((B, 2 ** 32 + 4), I32))
+    with pytest.raises(ValueError, match="2\\^31"):
+        call("attn", t)
+    long = (B, KVH, 2 ** 32 + CAP)
+    with pytest.raises(ValueError, match="2\\^31"):
+        call("weights", tensors("weights", acc=Fake(long, F32)))
+    with pytest.raises(ValueError, match="2\\^31"):
+        call("evict", tensors("evict", acc=Fake(long, F32), pos=Fake(long, I32), acc_out=Fake(long, F32), pos_out=Fake(long, I32)))
+    assert not [c for c in lib.calls if not c[0].endswith("bytes")]

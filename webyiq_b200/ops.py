@@ -323,6 +323,8 @@ class PagedKV(_Fixed):
             raise ValueError("PagedKV takes k and v [pages, KVH, page, D] of one type, float16 or bfloat16")
         if k.stride() != v.stride() or k.stride(3) != 1:
             raise ValueError("PagedKV takes k and v of the same strides, with inner stride 1")
+        if (k.stride(1) | k.stride(2)) >> 31:
+            raise ValueError("PagedKV takes strides of heads and slots below 2^31 elements")
         pages, KVH, page, D = k.shape
         self.__dict__.update(
             k=k, v=v, pages=pages, KVH=KVH, page=page, D=D, dtype=k.dtype, device=k.device, index=k.get_device(),
@@ -343,6 +345,16 @@ class PagedBatch(_Fixed):
 
     free = ("max_q", "max_kv")
 
+    def __setattr__(self, name, value):
+        super().__setattr__(name, self._bound(value) if name in self.free else value)
+
+    @staticmethod
+    def _bound(value):
+        value = int(value)
+        if value >> 31:
+            raise ValueError(f"PagedBatch: a bound of {value}, not in 0 .. 2^31 - 1")
+        return value
+
     def __init__(self, q_start, kv_len, table, max_q, max_kv):
         _need_cuda(q_start, kv_len, table)
         index, B = q_start.get_device(), kv_len.numel()
@@ -352,9 +364,11 @@ class PagedBatch(_Fixed):
             raise ValueError("PagedBatch takes int32 tensors")
         if q_start.numel() != B + 1 or table.dim() != 2 or table.shape[0] != B:
             raise ValueError("PagedBatch takes q_start [B + 1], kv_len [B] and table [B, pages a sequence]")
+        if table.shape[1] >> 31:
+            raise ValueError("PagedBatch takes fewer than 2^31 pages a sequence")
         self.__dict__.update(
-            q_start=q_start, kv_len=kv_len, table=table, max_q=int(max_q), max_kv=int(max_kv), B=B, per=table.shape[1],
-            index=index, pq=q_start.data_ptr(), pl=kv_len.data_ptr(), pt=table.data_ptr(),
+            q_start=q_start, kv_len=kv_len, table=table, max_q=self._bound(max_q), max_kv=self._bound(max_kv), B=B,
+            per=table.shape[1], index=index, pq=q_start.data_ptr(), pl=kv_len.data_ptr(), pt=table.data_ptr(),
             at=(q_start.data_ptr(), kv_len.data_ptr(), table.data_ptr()),
             now=(q_start.data_ptr, kv_len.data_ptr, table.data_ptr))
 
@@ -408,7 +422,11 @@ def _token_stride(name, t, kv):
     s = t.stride()
     if T * H and (s[2] != 1 or (s[1] != D and H > 1)):
         raise ValueError(f"{name}: contiguous within a token")
-    return s[0] if T > 1 else H * D
+    if T < 2:
+        return H * D
+    if s[0] >> 31:
+        raise ValueError(f"{name}: {s[0]} elements from token to token, not below 2^31")
+    return s[0]
 
 
 def qk_norm_rope_kv(qkv, kv, batch, pos, rope, H, q_norm=None, k_norm=None, eps=1e-6, gated=False, interleaved=False,
@@ -428,6 +446,10 @@ def qk_norm_rope_kv(qkv, kv, batch, pos, rope, H, q_norm=None, k_norm=None, eps=
     row, inner = qkv.stride()
     if width != H * qhs + 2 * kv.KVH * D or (inner != 1 and T):
         raise ValueError(f"qk_norm_rope_kv: rows of {width} for {H} query and {kv.KVH} kv heads of {D}, inner stride 1")
+    if T < 2:
+        row = width
+    elif row >> 31:
+        raise ValueError(f"qk_norm_rope_kv: {row} elements from row to row, not below 2^31")
     pqn, pkn = _opt(q_norm, torch.float32, "q_norm", at), _opt(k_norm, torch.float32, "k_norm", at)
     if (pqn and q_norm.numel() != D) or (pkn and k_norm.numel() != D):
         raise ValueError("qk_norm_rope_kv: norm weights f32 [D]")
@@ -442,7 +464,7 @@ def qk_norm_rope_kv(qkv, kv, batch, pos, rope, H, q_norm=None, k_norm=None, eps=
     elif q.shape != (T, H, D) or not _is(q, kv.dtype, at):
         raise ValueError("qk_norm_rope_kv: q [tokens, H, D] of the cache's type, contiguous")
     st = _lib.load().w4a8_qk_norm_rope_kv(
-        qkv.data_ptr(), row if T > 1 else width, qhs, H, kv.KVH, D, pqn, pkn, eps, prope, rot, rows, interleaved, ppos,
+        qkv.data_ptr(), row, qhs, H, kv.KVH, D, pqn, pkn, eps, prope, rot, rows, interleaved, ppos,
         batch.pq, batch.pl, batch.pt, batch.B, batch.per, T, q.data_ptr(), kv.pk, kv.pv, *kv.layout, _raw_stream(at))
     if st:
         _lib.check(st)
@@ -478,6 +500,8 @@ def attn_paged(q, kv, batch, scale=None, gate=None, o=None, lse=None, workspace=
         if gate.dtype is not torch.float32 or gate.shape != q.shape or gate.get_device() != at or gs[2] != 1:
             raise ValueError("attn_paged: gate f32 [tokens, H, D] with inner stride 1")
         pg, gr, gh = gate.data_ptr(), gs[0], gs[1]
+        if (gr | gh) >> 31:
+            raise ValueError("attn_paged: gate strides not below 2^31 elements")
     if workspace is None:
         workspace = attn_paged_workspace(batch, T, H, kv.KVH, D, kv.device)
     elif not _is(workspace, torch.uint8, at):
@@ -508,6 +532,8 @@ def attn_weights(q, lse, kv, batch, acc, scale=None, workspace=None):
         raise ValueError("attn_weights: lse f32 [tokens, H], contiguous")
     if acc.dim() != 3 or acc.shape[0] != batch.B or acc.shape[1] != kv.KVH or not _is(acc, torch.float32, at):
         raise ValueError("attn_weights: acc f32 [B, KVH, slots], contiguous")
+    if acc.shape[2] >> 31:
+        raise ValueError("attn_weights: fewer than 2^31 weights a head")
     if workspace is None:
         workspace = attn_weights_workspace(batch, H, kv.KVH, kv.device)
     st = _lib.load().w4a8_attn_weights(
@@ -537,8 +563,8 @@ def kv_evict(kv, batch, acc, pos, keep, protect_from, sink=0, acc_out=None, pos_
     if len(shape) != 3 or shape[0] != batch.B or shape[1] != kv.KVH:
         raise ValueError("kv_evict: acc f32 and pos int32 [B, KVH, slots], contiguous")
     slots = shape[2]
-    if slots < batch.max_kv:
-        raise ValueError(f"kv_evict: {slots} weights a head for up to {batch.max_kv} slots")
+    if slots < batch.max_kv or slots >> 31:
+        raise ValueError(f"kv_evict: {slots} weights a head for up to {batch.max_kv} slots (fewer than 2^31)")
     if acc_out is None:
         acc_out = acc
     if pos_out is None:

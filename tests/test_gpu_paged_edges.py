@@ -200,3 +200,26 @@ def test_evict_length_over_a_limit(cuda, over):
             for h in range(KVH):
                 best = np.argsort(-acc[b, h, :low], kind="stable")[:150 + b - 60 - b]
                 assert sorted(p[b, h, :150 + b].tolist()) == sorted([*best.tolist(), *range(low, L)])
+
+
+@pytest.mark.parametrize("T,H", [(1, 8), (5, 1), (1, 1)])
+def test_gate_strides_of_one(cuda, T, H):
+    """A dimension of one has no stride: whatever the gate's tensor gives for it is taken."""
+    c = Case(cuda, [77], [T], H, 1, 64, seed=T)
+    row, head = 3 if T == 1 else 64 * H + 4, 7 if H == 1 else 64
+    buf = torch.randn(T * (64 * H + 8) + 16, device=cuda)
+    gate = buf.as_strided((T, H, 64), (row, head, 1))
+    o, lse = ops.attn_paged(c.q, c.kv, c.batch, gate=gate)
+    c.check(o, lse, gate=gate.cpu().numpy())
+
+
+def test_cache_strides_of_one(cuda):
+    """One kv head and one page: whatever strides the tensors give for those dimensions, each its own."""
+    c = Case(cuda, [100], [9], 4, 1, 64, page=112)
+    one = int(c.table[0, 0])
+    k = torch.empty(112 * 64, dtype=c.k.dtype, device=cuda).as_strided((1, 1, 112, 64), (3, 5, 64, 1))
+    v = torch.empty(112 * 64, dtype=c.k.dtype, device=cuda).as_strided((1, 1, 112, 64), (7, 2 ** 40, 64, 1))
+    k.copy_(c.k[one:one + 1])
+    v.copy_(c.v[one:one + 1])
+    batch = ops.PagedBatch(c.batch.q_start, c.batch.kv_len, torch.zeros_like(c.batch.table), 9, 100)
+    c.check(*ops.attn_paged(c.q, ops.PagedKV(k, v), batch))

@@ -224,3 +224,14 @@ def test_refuses_sizes_past_31_bits(lib):
     with pytest.raises(ValueError, match="2\\^31"):
         call("evict", tensors("evict", acc=Fake(long, F32), pos=Fake(long, I32), acc_out=Fake(long, F32), pos_out=Fake(long, I32)))
     assert not [c for c in lib.calls if not c[0].endswith("bytes")]
+
+
+def test_dimensions_of_one_have_no_stride(lib):
+    """What a tensor gives as the stride of a dimension of one is not looked at, nor has to fit."""
+    t = tensors("attn", k=Fake((1, 1, PAGE, D), F16, stride=(3, 2 ** 40, D, 1)), v=Fake((1, 1, PAGE, D), F16, stride=(9, 5, D, 1)))
+    t["q"], t["o"] = Fake((1, 1, D), F16, stride=(7, 2 ** 33, 1)), Fake((1, 1, D), F16)
+    t["gate"], t["lse"] = Fake((1, 1, D), F32, stride=(3, 2 ** 35, 1)), Fake((1, 1), F32)
+    call("attn", t)
+    (_, args), = lib.calls
+    assert args[7:9] == (0, 0) and args[1] == D  # gate strides, q's row
+    assert args[22:25] == (0, 0, D)              # pages, heads, slots

@@ -321,15 +321,17 @@ class PagedKV(_Fixed):
             raise ValueError("PagedKV takes two tensors of one CUDA device")
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in (torch.float16, torch.bfloat16):
             raise ValueError("PagedKV takes k and v [pages, KVH, page, D] of one type, float16 or bfloat16")
-        if k.stride() != v.stride() or k.stride(3) != 1:
+        # (a dimension of one has no stride)
+        strides, of_v = ([s if n > 1 else 0 for n, s in zip(k.shape[:3], x.stride())] for x in (k, v))
+        if strides != of_v or k.stride(3) != 1 or v.stride(3) != 1:
             raise ValueError("PagedKV takes k and v of the same strides, with inner stride 1")
-        if (k.stride(1) | k.stride(2)) >> 31:
+        if (strides[1] | strides[2]) >> 31:
             raise ValueError("PagedKV takes strides of heads and slots below 2^31 elements")
         pages, KVH, page, D = k.shape
         self.__dict__.update(
             k=k, v=v, pages=pages, KVH=KVH, page=page, D=D, dtype=k.dtype, device=k.device, index=k.get_device(),
             scale=1.0 / math.sqrt(D),  # of the scores, where a call gives none
-            layout=(_TYPES[k.dtype], pages, page, k.stride(0), k.stride(1), k.stride(2)),
+            layout=(_TYPES[k.dtype], pages, page, *strides),
             pk=k.data_ptr(), pv=v.data_ptr(), at=(k.data_ptr(), v.data_ptr()), now=(k.data_ptr, v.data_ptr))
 
     def __repr__(self):
@@ -499,7 +501,7 @@ def attn_paged(q, kv, batch, scale=None, gate=None, o=None, lse=None, workspace=
         gs = gate.stride()
         if gate.dtype is not torch.float32 or gate.shape != q.shape or gate.get_device() != at or gs[2] != 1:
             raise ValueError("attn_paged: gate f32 [tokens, H, D] with inner stride 1")
-        pg, gr, gh = gate.data_ptr(), gs[0], gs[1]
+        pg, gr, gh = gate.data_ptr(), gs[0] if T > 1 else 0, gs[1] if H > 1 else 0
         if (gr | gh) >> 31:
             raise ValueError("attn_paged: gate strides not below 2^31 elements")
     if workspace is None:

@@ -329,7 +329,11 @@ W4A8_API w4a8_status w4a8_deltanet(const float* proj, const float* conv_w, float
  * taken from them (a start to tokens, a length to table_stride * page, a page to pages):
  * a wrong entry gives wrong values and no access out of range.  max_q and max_kv bound
  * the new tokens and slots of any sequence: new tokens past max_q are not computed,
- * max_kv only sizes the launch.  Slots past a sequence's length may hold anything, NaN
+ * max_kv only sizes the launch.  Sequences may share pages (a common prefix) where a
+ * call only reads them: attention and weights.  What it writes has to be a sequence's
+ * own: the pages of its new slots (append), all pages of its slots (eviction, which moves
+ * rows in place for each sequence on its own: a shared page would be changed under the
+ * others, by several at once); copy a shared page first.  Slots past a sequence's length may hold anything, NaN
  * too.  tokens = 0 is a no-op.  The row tiles (128 query rows of a kv head) of a call
  * times the 128-slot tiles each sees stay below 2^31 in all: past that a call computes
  * nothing and records code 32 in the device error word. */

@@ -341,7 +341,8 @@ class PagedKV(_Fixed):
 class PagedBatch(_Fixed):
     """A step's batch over a PagedKV: q_start int32 [B + 1] (first new token of each sequence,
     from 0), kv_len int32 [B] (slots, the new tokens' own among them), table int32 [B, pages a
-    sequence].  max_q and max_kv bound the new tokens and the slots of any sequence (read on
+    sequence]; sequences may share pages that a call only reads (kv_evict writes to all of its
+    sequences' pages, qk_norm_rope_kv to those of the new slots).  max_q and max_kv bound the new tokens and the slots of any sequence (read on
     the device otherwise, so the arrays may be rewritten in place between calls); the two may
     be assigned anew.  Holds the arrays' addresses, as PagedKV does."""
 

@@ -309,34 +309,34 @@ W4A8_API w4a8_status w4a8_deltanet(const float* proj, const float* conv_w, float
                                    const uint32_t* params, int32_t nh, int32_t m, float eps, int32_t spec,
                                    void* stream);
 
-/* Paged KV cache of a batch of sequences, and the operators on it: the q/k norm with
- * the rotation and the append (rope_kv.wgsl, qk_norm_rope.wgsl), attention of new tokens
- * (attn.wgsl, attn_prefill.wgsl for one sequence and a contiguous cache), the weight that
- * cached slots received, and eviction by that weight (the last two have no counterpart
- * in the reference).
- *
+/* Paged KV cache of a batch of sequences, and the operators on it: the q/k norm with the
+ * rotation and the append (rope_kv.wgsl, qk_norm_rope.wgsl), attention of new tokens
+ * (attn.wgsl, attn_prefill.wgsl for one sequence and a contiguous cache), the weight
+ * that cached slots received, and eviction by that weight (the last two have no
+ * counterpart in the reference).
  * Cache: k, v [pages, KVH, page, D] of type dtype, each with the strides page_stride,
  * head_stride, row_stride (in elements, multiples of 8; unit inner stride; any order of
  * the dimensions in memory, nothing overlapping), 16-byte aligned.  page: slots a page,
  * a multiple of 16 up to 1024.  D: a multiple of 16 up to 256.  H query heads, H / KVH
  * (at most 128) for each kv head, consecutive.
- * Batch: sequence b has the new tokens q_start[b] .. q_start[b + 1] (q_start u32[batch + 1],
- * q_start[0] = 0, at most `tokens` in all) and kv_len[b] slots, the new tokens' own among
- * them: the last ones.  Slot j is row j % page of page table[b, j / page] (table
- * u32[batch, table_stride]; entries past the length are not read).  New token i of n sees
- * slots 0 .. kv_len - n + i, none where that is negative.  The arrays are read on the
- * device, so a captured graph replays for new contents; the kernels bound every index
- * taken from them (a start to tokens, a length to table_stride * page, a page to pages):
- * a wrong entry gives wrong values and no access out of range.  max_q and max_kv bound
- * the new tokens and slots of any sequence: new tokens past max_q are not computed,
- * max_kv only sizes the launch.  Sequences may share pages (a common prefix) where a
- * call only reads them: attention and weights.  What it writes has to be a sequence's
- * own: the pages of its new slots (append), all pages of its slots (eviction, which moves
- * rows in place for each sequence on its own: a shared page would be changed under the
- * others, by several at once); copy a shared page first.  Slots past a sequence's length may hold anything, NaN
- * too.  tokens = 0 is a no-op.  The row tiles (128 query rows of a kv head) of a call
- * times the 128-slot tiles each sees stay below 2^31 in all: past that a call computes
- * nothing and records code 32 in the device error word. */
+ * Batch: sequence b has the new tokens q_start[b] .. q_start[b + 1] (q_start u32[batch +
+ * 1], q_start[0] = 0, at most `tokens` in all) and kv_len[b] slots, the new tokens' own
+ * among them: the last ones.  Slot j is row j % page of page table[b, j / page] (table
+ * u32[batch, table_stride]; entries past the length are not read).  New token i of n
+ * sees slots 0 .. kv_len - n + i, none where that is negative.  The arrays are read on
+ * the device, so a captured graph replays for new contents; the kernels bound every
+ * index taken from them (a start to tokens, a length to table_stride * page, a page to
+ * pages): a wrong entry gives wrong values and no access out of range.  max_q and max_kv
+ * bound the new tokens and slots of any sequence: new tokens past max_q are not
+ * computed, max_kv only sizes the launch.  Sequences may share pages (a common prefix)
+ * where a call only reads them: attention and weights.  What it writes has to be a
+ * sequence's own: the pages of its new slots (append), all pages of its slots (eviction,
+ * which moves rows in place for each sequence on its own: a shared page would be changed
+ * under the others, by several at once); copy a shared page first.  Slots past a
+ * sequence's length may hold anything, NaN too.  tokens = 0 is a no-op.  The row tiles
+ * (128 query rows of a kv head) of a call times the 128-slot tiles each sees stay below
+ * 2^31 in all: past that a call computes nothing and records code 32 in the device error
+ * word. */
 enum { W4A8_F16 = 0, W4A8_BF16 = 1, W4A8_F32 = 2 };
 
 /* Norm of queries and keys per head, rotation, and append to the cache, in one pass over
@@ -360,15 +360,17 @@ W4A8_API w4a8_status w4a8_qk_norm_rope_kv(const float* qkv, int32_t qkv_row_stri
 
 /* Attention of the batch's new tokens over the cache: softmax(scale q k^T) v over the
  * slots each token sees, times sigmoid(gate) where gate is given.  q [tokens, H, D] of
- * the cache's type, q_row_stride elements a token (a multiple of 8); gate f32, element
- * t * gate_row_stride + h * gate_head_stride + d; o [tokens, H, D] of type o_type (the
+ * the cache's type, q_row_stride elements a token (a multiple of 8); gate f32, element t
+ * * gate_row_stride + h * gate_head_stride + d; o [tokens, H, D] of type o_type (the
  * cache's, or W4A8_F32); lse f32[tokens, H] (natural log of the sum of exp(scale q k^T))
  * or NULL.  A token that sees nothing gets o = 0 and lse = -inf.  Scores, sums and
- * accumulators are f32; the weights are rounded to the cache's type before they
- * meet v (f16: to 2^-11 of a weight, or to 2^-32 of the row's largest where that is more).  k and v must be finite in the slots below a sequence's length: a weight of
- * zero times an infinity is NaN.
- * workspace: w4a8_attn_paged_workspace_bytes(...) bytes (of the current device), 16-byte
- * aligned, any contents; calls that share one must not overlap on the GPU. */
+ * accumulators are f32; the weights are rounded to the cache's type before they meet v
+ * (f16: to 2^-11 of a weight, or to 2^-32 of the row's largest where that is more).  k
+ * and v must be finite in the slots below a sequence's length: a weight of zero times an
+ * infinity is NaN.
+ * workspace: w4a8_attn_paged_workspace_bytes(...) bytes (of the current device; the
+ * number of tokens does not change them), 16-byte aligned, any contents; calls that
+ * share one must not overlap on the GPU. */
 W4A8_API w4a8_status w4a8_attn_paged(const void* q, int32_t q_row_stride, int32_t H, int32_t KVH, int32_t D, float scale,
                                      const float* gate, int32_t gate_row_stride, int32_t gate_head_stride,
                                      const uint32_t* q_start, const uint32_t* kv_len, const uint32_t* table,
@@ -396,15 +398,16 @@ W4A8_API w4a8_status w4a8_attn_weights(const void* q, int32_t q_row_stride, cons
 W4A8_API size_t w4a8_attn_weights_workspace_bytes(int32_t H, int32_t KVH, int32_t max_q);
 
 /* Eviction by accumulated weight, for each sequence and kv head on its own: of len =
- * kv_len[b] slots the n = min(len, keep[b]) stay that come first: the
- * protected ones by slot, the lower first, then by weight acc, the larger first (the lower
- * slot among equals; NaN ranks as the lowest weight, and +inf protects nothing); a slot is protected where its
- * token's position pos (u32[batch, KVH, stride], as acc) is below sink or at least
- * protect_from[b].  The i-th kept slot at n or past it moves into the i-th dropped slot
- * below n, K and V rows, weight and position; every other slot stays where it is
- * (keys carry their rotation, so the order of slots has no meaning).  acc_out and pos_out
- * get the first n entries of each head (they may be acc and pos); len_out[b] = n
- * (not kv_len itself; keep or protect_from will do).  stride >= any kv_len.
+ * kv_len[b] slots the n = min(len, keep[b]) stay that come first: the protected ones by
+ * slot, the lower first, then by weight acc, the larger first (the lower slot among
+ * equals; NaN ranks as the lowest weight, and +inf protects nothing); a slot is
+ * protected where its token's position pos (u32[batch, KVH, stride], as acc) is below
+ * sink or at least protect_from[b].  The i-th kept slot at n or past it moves into the
+ * i-th dropped slot below n, K and V rows, weight and position; every other slot stays
+ * where it is (keys carry their rotation, so the order of slots has no meaning).
+ * acc_out and pos_out get the first n entries of each head (they may be acc and pos);
+ * len_out[b] = n (not kv_len itself; keep or protect_from will do).  stride >= any
+ * kv_len.
  * workspace: w4a8_kv_evict_workspace_bytes(...) bytes, 16-byte aligned, any contents;
  * calls that share one must not overlap on the GPU. */
 W4A8_API w4a8_status w4a8_kv_evict(void* k, void* v, int32_t dtype, int32_t pages, int32_t page, size_t page_stride,
@@ -413,10 +416,10 @@ W4A8_API w4a8_status w4a8_kv_evict(void* k, void* v, int32_t dtype, int32_t page
                                    const float* acc, const uint32_t* pos, int32_t stride, const uint32_t* keep,
                                    const uint32_t* protect_from, int32_t sink, float* acc_out, uint32_t* pos_out,
                                    uint32_t* len_out, void* workspace, size_t workspace_bytes, void* stream);
-/* The same for limits in two's complement, as a host with signed 32-bit arrays computes them: a
- * protect_from at or below zero (seen - window of a sequence shorter than its window) protects
- * every slot, a keep below zero keeps none.  w4a8_kv_evict takes such entries as values from 2^31
- * on, which protect nothing and keep everything. */
+/* The same for limits in two's complement, as a host with signed 32-bit arrays computes
+ * them: a protect_from at or below zero (seen - window of a sequence shorter than its
+ * window) protects every slot, a keep below zero keeps none.  w4a8_kv_evict takes such
+ * entries as values from 2^31 on, which protect nothing and keep everything. */
 W4A8_API w4a8_status w4a8_kv_evict_signed(void* k, void* v, int32_t dtype, int32_t pages, int32_t page,
                                           size_t page_stride, int32_t head_stride, int32_t row_stride, int32_t KVH,
                                           int32_t D, const uint32_t* kv_len, const uint32_t* table, int32_t batch,

@@ -109,7 +109,7 @@ struct AttnParams {
     void* o;
     int o_type;
     float* lse;
-    int max_q, max_kv;
+    int max_q;
     int item_cost;   // kItemCost or kGatedItemCost
     int box_rows;    // slots of a TMA box
     int box_tokens;  // tokens of one
@@ -1289,7 +1289,7 @@ extern "C" {
 
 W4A8_API size_t w4a8_attn_paged_workspace_bytes(int32_t tokens, int32_t H, int32_t KVH, int32_t D, int32_t batch,
                                                 int32_t max_q, int32_t max_kv) {
-    (void)tokens;
+    (void)tokens;  // partial results are a CTA's, not a token's
     if (check_heads("w4a8_attn_paged_workspace_bytes", H, KVH, D) != W4A8_OK || batch < 1 || max_q < 0 || max_kv < 0)
         return 0;
     return layout_of(H, KVH, D, batch, max_q, max_kv, sm_count()).bytes;
@@ -1341,7 +1341,6 @@ W4A8_API w4a8_status w4a8_attn_paged(const void* q, int32_t q_row_stride, int32_
     p.o_type = o_type;
     p.lse = lse;
     p.max_q = max_q;
-    p.max_kv = max_kv;
     p.item_cost = gate ? kGatedItemCost : kItemCost;
     p.box_rows = std::min(cache_box_rows(page), x.pair ? kTile / 2 : kTile);  // a pair's CTA takes 64 slots of K
     p.box_tokens = std::min(x.tpt, max_q);

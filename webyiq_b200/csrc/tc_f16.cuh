@@ -1,6 +1,6 @@
-// One-SM tcgen05 helpers for 16-bit operands, shared by the attention kernels: tensor
-// memory, descriptors of 128-byte-swizzled tiles, kind::f16 MMAs, and the tensor map of
-// a paged cache or of query rows.  No load here uses cluster multicast.
+// tcgen05 helpers for 16-bit operands, of one SM and of pairs, shared by the attention
+// kernels: tensor memory, descriptors of 128-byte-swizzled tiles, kind::f16 MMAs, the tensor
+// maps of a paged cache and of query rows, places on a work line, and bounded waits.  No load here uses cluster multicast.
 #pragma once
 
 #include <cuda.h>

@@ -64,7 +64,7 @@ class Library:
 
     def __getattr__(self, name):
         def call(*args):
-            self.calls.append((name, args))
+            self.calls.append((name, tuple(getattr(a, "value", a) for a in args)))
             return 0
         return call
 

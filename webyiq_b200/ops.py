@@ -328,11 +328,15 @@ class PagedKV(_Fixed):
         if (strides[1] | strides[2]) >> 31:
             raise ValueError("PagedKV takes strides of heads and slots below 2^31 elements")
         pages, KVH, page, D = k.shape
+        layout = (_TYPES[k.dtype], pages, page, *strides)
+        # the library's arguments, converted once: a call of some thirty spends 3 us on that
+        sizes = [ty(x) for ty, x in zip((ctypes.c_int32,) * 3 + (ctypes.c_size_t,) + (ctypes.c_int32,) * 2, layout)]
+        pk, pv = _ptr(k), _ptr(v)
         self.__dict__.update(
             k=k, v=v, pages=pages, KVH=KVH, page=page, D=D, dtype=k.dtype, device=k.device, index=k.get_device(),
             scale=1.0 / math.sqrt(D),  # of the scores, where a call gives none
-            layout=(_TYPES[k.dtype], pages, page, *strides),
-            pk=k.data_ptr(), pv=v.data_ptr(), at=(k.data_ptr(), v.data_ptr()), now=(k.data_ptr, v.data_ptr))
+            layout=layout, c=(pk, pv, *sizes), c_k=(pk, *sizes), at=(k.data_ptr(), v.data_ptr()),
+            now=(k.data_ptr, v.data_ptr))
 
     def __repr__(self):
         return f"PagedKV(pages={self.pages}, KVH={self.KVH}, page={self.page}, D={self.D}, {self.dtype})"
@@ -369,9 +373,10 @@ class PagedBatch(_Fixed):
             raise ValueError("PagedBatch takes q_start [B + 1], kv_len [B] and table [B, pages a sequence]")
         if table.shape[1] >> 31:
             raise ValueError("PagedBatch takes fewer than 2^31 pages a sequence")
+        c = (_ptr(q_start), _ptr(kv_len), _ptr(table), ctypes.c_int32(B), ctypes.c_int32(table.shape[1]))
         self.__dict__.update(
             q_start=q_start, kv_len=kv_len, table=table, max_q=self._bound(max_q), max_kv=self._bound(max_kv), B=B,
-            per=table.shape[1], index=index, pq=q_start.data_ptr(), pl=kv_len.data_ptr(), pt=table.data_ptr(),
+            per=table.shape[1], index=index, c=c, c_slots=c[1:],
             at=(q_start.data_ptr(), kv_len.data_ptr(), table.data_ptr()),
             now=(q_start.data_ptr, kv_len.data_ptr, table.data_ptr))
 
@@ -468,7 +473,7 @@ def qk_norm_rope_kv(qkv, kv, batch, pos, rope, H, q_norm=None, k_norm=None, eps=
         raise ValueError("qk_norm_rope_kv: q [tokens, H, D] of the cache's type, contiguous")
     st = _lib.load().w4a8_qk_norm_rope_kv(
         qkv.data_ptr(), row, qhs, H, kv.KVH, D, pqn, pkn, eps, prope, rot, rows, interleaved, ppos,
-        batch.pq, batch.pl, batch.pt, batch.B, batch.per, T, q.data_ptr(), kv.pk, kv.pv, *kv.layout, _raw_stream(at))
+        *batch.c, T, q.data_ptr(), *kv.c, _raw_stream(at))
     if st:
         _lib.check(st)
     return q
@@ -510,8 +515,8 @@ def attn_paged(q, kv, batch, scale=None, gate=None, o=None, lse=None, workspace=
     elif not _is(workspace, torch.uint8, at):
         raise ValueError("attn_paged: workspace uint8")
     st = _lib.load().w4a8_attn_paged(
-        q.data_ptr(), row, H, kv.KVH, D, kv.scale if scale is None else scale, pg, gr, gh, batch.pq, batch.pl, batch.pt,
-        batch.B, batch.per, T, batch.max_q, batch.max_kv, kv.pk, kv.pv, *kv.layout, o.data_ptr(), _TYPES.get(o.dtype, -1),
+        q.data_ptr(), row, H, kv.KVH, D, kv.scale if scale is None else scale, pg, gr, gh, *batch.c, T,
+        batch.max_q, batch.max_kv, *kv.c, o.data_ptr(), _TYPES.get(o.dtype, -1),
         lse.data_ptr(), workspace.data_ptr(), workspace.numel(), _raw_stream(at))
     if st:
         _lib.check(st)
@@ -540,8 +545,8 @@ def attn_weights(q, lse, kv, batch, acc, scale=None, workspace=None):
     if workspace is None:
         workspace = attn_weights_workspace(batch, H, kv.KVH, kv.device)
     st = _lib.load().w4a8_attn_weights(
-        q.data_ptr(), row, lse.data_ptr(), H, kv.KVH, D, kv.scale if scale is None else scale, batch.pq, batch.pl, batch.pt,
-        batch.B, batch.per, T, batch.max_q, batch.max_kv, kv.pk, *kv.layout, acc.data_ptr(), acc.shape[2],
+        q.data_ptr(), row, lse.data_ptr(), H, kv.KVH, D, kv.scale if scale is None else scale, *batch.c, T,
+        batch.max_q, batch.max_kv, *kv.c_k, acc.data_ptr(), acc.shape[2],
         _opt(workspace, torch.uint8, "workspace", at), 0 if workspace is None else workspace.numel(), _raw_stream(at))
     if st:
         _lib.check(st)
@@ -585,9 +590,9 @@ def kv_evict(kv, batch, acc, pos, keep, protect_from, sink=0, acc_out=None, pos_
     elif not _is(workspace, torch.uint8, at):
         raise ValueError("kv_evict: workspace uint8")
     st = _lib.load().w4a8_kv_evict_signed(
-        kv.pk, kv.pv, *kv.layout, kv.KVH, kv.D, batch.pl, batch.pt, batch.B, batch.per, acc.data_ptr(), pos.data_ptr(),
-        slots, keep.data_ptr(), protect_from.data_ptr(), sink, acc_out.data_ptr(), pos_out.data_ptr(), len_out.data_ptr(),
-        workspace.data_ptr(), workspace.numel(), _raw_stream(at))
+        *kv.c, kv.KVH, kv.D, *batch.c_slots, acc.data_ptr(), pos.data_ptr(), slots, keep.data_ptr(), protect_from.data_ptr(),
+        sink, acc_out.data_ptr(), pos_out.data_ptr(), len_out.data_ptr(), workspace.data_ptr(), workspace.numel(),
+        _raw_stream(at))
     if st:
         _lib.check(st)
     return acc_out, pos_out, len_out

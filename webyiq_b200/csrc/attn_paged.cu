@@ -36,8 +36,9 @@
 //  - Two threads issue MMAs, each for its own S buffers: a thread that waits or commits
 //    holds up its own MMAs only.
 //
-// What bounds it, measured: 2048 tokens over 16384 slots, 32 / 8 heads of 128: 446 us in
-// short runs, 1157 TFLOP/s (0.69 of the measured bf16 burst rate), more at the 1000 W limit.
+// What bounds it, measured: 2048 tokens over 16384 slots, 32 / 8 heads of 128: 446 to 480 us
+// in short runs, at best 1157 TFLOP/s (0.69 of the measured bf16 burst rate), 521 to 534 back to
+// back at the 1000 W limit.
 // Not one unit but the hand-overs between them: a warp's 64 exponentials take 512 clocks at
 // the unit's rate (611 with their sums and rounding), its half step about 1900, and S is ready in 99
 // of 100 half steps; heads of 64, with two thirds of the MMAs, still take 412 us.  An MMA
@@ -48,9 +49,12 @@
 // multiplies, exponentials, sums and roundings: no change.)  256-wide heads: 2048 tokens over 16384
 // slots, 8 / 2 heads, in 247 us as pairs, 1044 TFLOP/s, and 276 as single CTAs, which read
 // 128 KB from L2 a step of 2048 clocks; a 4001-token prompt 90 against 100, gated 113
-// against 117; now 87 and 109.
-// Single tokens: 48 sequences, 888 MB, at 5.5 to 6.0 TB/s (0.84 to 0.92 of the measured copy
-// rate); one token over 100003 slots 46.6 us, 15 above its
+// against 117; now 87 to 91 and 107 to 109.  Heads of 129 to 192 take single CTAs whatever the
+// rows (96 KB a step of 1536 clocks): 1024 tokens over 8192 slots, 32 / 8 heads of 192, in 181 us,
+// 1068 TFLOP/s, nearer the burst rate than 256-wide pairs (262 us, 983) and 128-wide double tiles
+// (138 us, 932).  Heads of 80 and 96 cost nearly what 128 do (131 and 134 us).
+// Single tokens: 48 sequences, 888 MB, at 5.9 TB/s in short runs (0.91 of the measured copy
+// rate), 5.0 to 5.3 back to back; one token over 100003 slots 47 to 50 us, 16 to 18 above its
 // bytes' time: the line, the first loads and the merge.
 //
 // Work split.  The kv steps of all (sequence, kv head, row tile) items lie on one line,

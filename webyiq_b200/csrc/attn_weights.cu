@@ -17,9 +17,9 @@
 // workspace, and a small kernel adds those in the order of the stretches.  Single tokens
 // are bound by HBM (K is read once), chunks by the exponentials: 128 x 128 of them take
 // the SM's 16 a clock 1024 clocks, the MMA half of that at 128-wide heads.  Measured: 1500
-// tokens over 8200 slots, 32 / 8 heads of 128, in 134 us (682 TFLOP/s, the
+// tokens over 8200 slots, 32 / 8 heads of 128, in 134 us at best, 139 to 142 usually (682 TFLOP/s, the
 // exponentials alone take 151 K clocks, 77 us at 1965 MHz; 182 with one MMA warp, whose barrier tests and commits left gaps, 251
-// with two softmax warpgroups); 16 single tokens over 56 MB in 17.6 us.
+// with two softmax warpgroups); 16 single tokens over 56 MB in 17.6 to 18.8 us.
 // (136 and 17.9 with the abort flag read before every wait, not only where one has to wait.)
 //
 // Warp roles: four softmax warpgroups that take row tiles in turn, an S buffer each, so

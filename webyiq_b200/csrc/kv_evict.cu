@@ -16,7 +16,7 @@
 // ties, the dropped slots below n and the kept slots past it.  (One CTA a head with the
 // keys read again for each of four 8-bit digits and a scan for every 1024 slots took 87 us
 // for 32 heads of 30011 slots, with 11-bit digits and one read 36 us; clusters of
-// 4 take 22 us, and the whole eviction to 4096 slots 39 to 41 us.)
+// 4 take 22 to 24 us, and the whole eviction to 4096 slots 39 to 42 us.)
 #include <cooperative_groups.h>
 
 #include <algorithm>
